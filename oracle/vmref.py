@@ -46,10 +46,10 @@ import numpy as np
 
 # --- format constants (independent restatement of docs/vmprogram.md) -----------
 MAGIC, VERSION = 0x314D5056, 3
-F32, I32, U32, BOOL, I64, F64, F16, BF16 = range(8)
+F32, I32, U32, BOOL, I64, F64, F16, BF16, I8 = range(9)      # I8: extension, pages of a paged cache
 NP = {F32: np.float32, I32: np.int32, U32: np.uint32, BOOL: np.uint8,
-      I64: np.int64, F64: np.float64, F16: np.float16, BF16: np.uint16}
-SIZE = {F32: 4, I32: 4, U32: 4, BOOL: 1, I64: 8, F64: 8, F16: 2, BF16: 2}
+      I64: np.int64, F64: np.float64, F16: np.float16, BF16: np.uint16, I8: np.int8}
+SIZE = {F32: 4, I32: 4, U32: 4, BOOL: 1, I64: 8, F64: 8, F16: 2, BF16: 2, I8: 1}
 INTS = (I32, U32, I64)
 
 NOP, BARRIER, WHILE, IF, FOR = (0xFFFFFFFF, 0xFFFFFFFE, 0xFFFFFFFD,
@@ -75,6 +75,11 @@ PINS = {
                    "inputs, and equal to the decomposed dot / mask / softmax / dot chain "
                    "of pinned ops with the cache column at pos holding k, v",
     "gather/scatter/dyn": "brute force index loops on tiny inputs",
+    "rotary": "extension without a reference counterpart: complex products in float64, and the "
+              "gradient against central differences",
+    "paged cache": "extension without a reference counterpart: brute-force loops over rows, "
+                   "positions and heads on tiny inputs, and equal to flash attention's closed form "
+                   "where one sequence fills its pages",
 }
 
 
@@ -138,6 +143,7 @@ class Prog:
     root_lens: list | None = None
     n_lanes: int = 0
     n_flags: int = 0
+    states: frozenset = frozenset()      # extension: inputs that tasks write in place
 
 
 def parse(data: bytes) -> Prog:
@@ -153,12 +159,15 @@ def parse(data: bytes) -> Prog:
     if hpad or main_len > ni:
         raise FormatError("bad header")
     pos = 48
-    bufs = []
+    bufs, states = [], set()
     for i in range(nb):
         off, size, dt, pad = struct.unpack_from("<QQII", data, pos)
         pos += 24
-        if off % 64 or off + size > arena or dt > BF16 or pad:
+        # pad 1 (extension): caller-owned memory, its offset past the arena
+        if off % 64 or (off < arena if pad == 1 else off + size > arena) or dt > I8 or pad > 1:
             raise FormatError(f"bad buffer {i}")
+        if pad:
+            states.add(i)
         bufs.append((off, size, dt))
 
     def al():
@@ -189,8 +198,10 @@ def parse(data: bytes) -> Prog:
     for _ in range(ni):
         instrs.append(struct.unpack_from("<8I", data, pos))
         pos += 32
+    if any(inputs.count(i) != 1 or i in outputs for i in states):
+        raise FormatError("a state buffer is an input of its own")
     p = Prog(arena, bufs, inputs, outputs, shapes[:nin], shapes[nin:], consts,
-             instrs, main_len, aux)
+             instrs, main_len, aux, states=frozenset(states))
     if pos < len(data):
         nt, ne, nf, nl = struct.unpack_from("<4I", data, pos)
         pos += 16
@@ -243,10 +254,13 @@ class Mem:
     def __init__(self, prog: Prog):
         self.p = prog
         self.arena = np.zeros(prog.arena_bytes + 64, np.uint8)
+        self.ext = {}                   # state buffer -> the caller's memory
 
     def view(self, bid, dt=None):
         off, size, bdt = self.p.bufs[bid]
         dt = bdt if dt is None else dt
+        if bid in self.ext:
+            return self.ext[bid].view(NP[dt])
         return self.arena[off:off + size].view(NP[dt])
 
     def load_f(self, bid, dt=None):
@@ -281,6 +295,12 @@ def _setup(prog: Prog, args) -> Mem:
         m.arena[off:off + len(data)] = np.frombuffer(data, np.uint8)
     for bid, arg in zip(prog.inputs, args):
         dt = prog.bufs[bid][2]
+        if bid in prog.states:          # in place: the caller's array itself
+            if not (isinstance(arg, np.ndarray) and arg.flags.c_contiguous and arg.dtype == NP[dt] and
+                    arg.nbytes == prog.bufs[bid][1]):
+                raise ValueError(f"state buffer {bid}: a contiguous {np.dtype(NP[dt])} array of {prog.bufs[bid][1]} bytes")
+            m.ext[bid] = arg.reshape(-1).view(np.uint8)
+            continue
         flat = np.ascontiguousarray(arg).reshape(-1)
         if dt == BF16 and flat.dtype != np.uint16:
             flat = f32_to_bf16(flat.astype(np.float32))
@@ -532,6 +552,99 @@ def decode_attention(q, Kt, Vc, k, v, pos, scale, krow=False, masked=False):
     out = np.einsum("hc,hcd->hd", e, vals)
     if masked and int(pos) < 0:
         out[:] = np.nan
+    return out
+
+
+def rotary(x, pos, freq_words, rot, interleaved, inverse, mag, weight=None, eps=0.0):
+    """Extension OP_ROTARY: x [T, H, hd] f64, pos [T], freq_words [rot / 2, 2] u32 (64-bit
+    fixed-point turns per position).  Each channel pair is a complex number times
+    mag e^(i angle); with a weight the head is first x / sqrt(mean x^2 + eps) * weight."""
+    x = x.astype(np.float64)
+    hd = x.shape[-1]
+    if weight is not None:
+        x = x / np.sqrt((x ** 2).sum(-1, keepdims=True) / hd + eps) * weight.astype(np.float64)
+    ang = rotary_angles(pos, freq_words)
+    unit = mag * np.exp(1j * (-ang if inverse else ang))[:, None, :]
+    y = x.copy()
+    a, b = (slice(0, rot, 2), slice(1, rot, 2)) if interleaved else (slice(0, rot // 2), slice(rot // 2, rot))
+    z = (x[..., a] + 1j * x[..., b]) * unit
+    y[..., a], y[..., b] = z.real, z.imag
+    return y
+
+
+def rotary_angles(pos, freq_words):
+    """[T, R] radians in [0, 2 pi): position times turns modulo one turn, in integers."""
+    ang = np.empty((len(pos), len(freq_words)))
+    for i, (lo, hi) in enumerate(freq_words):
+        w = int(hi) << 32 | int(lo)
+        ang[:, i] = [((int(p) * w) & ((1 << 64) - 1)) / 2.0 ** 64 * 2 * np.pi for p in pos]
+    return ang
+
+
+def rotary_grad(dy, x, pos, freq_words, rot, interleaved, mag, weight, eps):
+    """(dx, dweight) of ``rotary`` with a norm: dz = R^T dy and u = x / rms give dweight =
+    sum dz u and dx = (g - u mean(g u)) / rms with g = dz weight."""
+    x = x.astype(np.float64)
+    dz = rotary(dy, pos, freq_words, rot, interleaved, True, mag)
+    rms = np.sqrt((x ** 2).sum(-1, keepdims=True) / x.shape[-1] + eps)
+    u = x / rms
+    g = dz * weight.astype(np.float64)
+    return (g - u * (g * u).mean(-1, keepdims=True)) / rms, (dz * u).sum((0, 1))
+
+
+def paged_rows(T, cu, lens, table, n_pages, page):
+    """[(row, sequence, position)] of the rows that belong to a sequence whose length
+    fits them and its pages."""
+    out = []
+    for s in range(len(lens)):
+        a, b = (min(max(int(c), 0), T) for c in cu[s:s + 2])
+        n, length = b - a, int(lens[s])
+        if n > 0 and n <= length <= table.shape[1] * page:
+            out += [(a + i, s, length - n + i) for i in range(n)]
+    return out
+
+
+def paged_place(table, s, p, n_pages, page):
+    """(page, slot) of position p of sequence s, None when its entry is no page."""
+    e = int(table[s, p // page])
+    return (e, p % page) if 0 <= e < n_pages else None
+
+
+def quantise_row(x):
+    """(int8 q, f32 scale) of one row: scale = max|x| / 127 in f32, q = rint(x / scale)."""
+    x = x.astype(np.float32)
+    if not np.isfinite(x).all():
+        return np.zeros(x.shape, np.int8), np.float32(np.nan)
+    scale = np.abs(x).max() * np.float32(1.0 / 127.0)
+    if not scale > 0:
+        return np.zeros(x.shape, np.int8), scale
+    return np.clip(np.rint(x / scale), -127, 127).astype(np.int8), scale
+
+
+def paged_attention(q, kv, cu, lens, table, n_pages, page, scale, window):
+    """q [T, Hq, hd] f64; kv(page, slot) -> (k, v) [Hkv, hd] f64.  One row and head at a
+    time over the positions it sees."""
+    T, Hq, hd = q.shape
+    out = np.zeros(q.shape)
+    held = {}
+    for r, s, p in paged_rows(T, cu, lens, table, n_pages, page):
+        ks, vs = [], []
+        for j in range(max(0, p + 1 - window) if window else 0, p + 1):
+            at = paged_place(table, s, j, n_pages, page)
+            if at is None:
+                continue
+            if at not in held:
+                held[at] = kv(*at)
+            ks.append(held[at][0])
+            vs.append(held[at][1])
+        if not ks:
+            continue
+        ks, vs = np.stack(ks, 1), np.stack(vs, 1)              # [Hkv, keys, hd]
+        g = Hq // ks.shape[0]
+        for h in range(Hq):
+            w = ks[h // g] @ q[r, h] * scale
+            e = np.exp(w - w.max())
+            out[r, h] = (e / e.sum()) @ vs[h // g]
     return out
 
 
@@ -1016,6 +1129,121 @@ class TaskRunner:
         o = decode_attention(q[sl], Kt[sl], Vc[sl], k[sl], v[sl], pos, float(_bits_f32(t.p[7])), krow, masked)
         self.m.store_f(t.dst, slice(h0 * hd, h1 * hd), o.reshape(-1).astype(np.float32), t.dt)
 
+    # 22, 23: rotary positions (extension).  A tile is four (row, head split) pairs; every
+    # row has been written once the last of its splits has run, whichever that is.
+    def _rows3(self, bid, dt, words, T, H, hd):
+        rs, hs, off = words
+        idx = off + np.arange(T)[:, None, None] * rs + np.arange(H)[None, :, None] * hs + np.arange(hd)
+        return self.m.load_f(bid, dt)[idx].astype(np.float64)
+
+    def top22(self, t, lo, hi):
+        m = self.m
+        T, H, hd, rot, flags, eps, mag, *st = m.aux_view(t.p[2], 13)
+        Z = t.p[3]
+        hz = -(-H // Z)
+        weight = m.load_f(t.b, F32)[:hd] if flags & 2 else None
+        pos = m.view(t.p[0], I32)[:T]
+        fw = m.view(t.p[1], U32)[:rot].reshape(-1, 2)
+        rows = sorted({u // Z for u in range(4 * lo, min(4 * hi, T * Z))})
+        if not rows:
+            return
+        y = rotary(self._rows3(t.a, t.adt, st[:3], T, H, hd)[rows], pos[rows], fw, rot, bool(flags & 1), bool(flags & 4),
+                   float(_bits_f32(mag & 0xFFFFFFFF)), weight, float(_bits_f32(eps & 0xFFFFFFFF)))
+        for u in range(4 * lo, min(4 * hi, T * Z)):
+            r, h0 = u // Z, u % Z * hz
+            h1 = min(H, h0 + hz)
+            if h0 < h1:
+                at = (r * H + h0) * hd
+                m.store_f(t.dst, slice(at, at + (h1 - h0) * hd), y[rows.index(r), h0:h1].reshape(-1), t.dt)
+
+    def top23(self, t, lo, hi):
+        m = self.m
+        T, H, hd, rot, flags, eps, mag, *st = m.aux_view(t.p[2], 13)
+        dy, x = self._rows3(t.a, t.adt, st[:3], T, H, hd), self._rows3(t.b, t.adt, st[3:6], T, H, hd)
+        pos = m.view(t.p[0], I32)[:T]
+        fw = m.view(t.p[1], U32)[:rot].reshape(-1, 2)
+        W = t.p[3]
+        w = m.load_f(t.p[4], F32)[:hd]
+        for tile in range(lo, hi):
+            a, b = T * H * tile // W, T * H * (tile + 1) // W
+            rows, heads = np.arange(a, b) // H, np.arange(a, b) % H
+            if b > a:
+                dx, dw = rotary_grad(dy[rows, heads][:, None], x[rows, heads][:, None], pos[rows], fw, rot,
+                                     bool(flags & 1), float(_bits_f32(mag & 0xFFFFFFFF)), w,
+                                     float(_bits_f32(eps & 0xFFFFFFFF)))
+                m.store_f(t.dst, slice(a * hd, b * hd), dx.reshape(-1), t.dt)
+            else:
+                dw = np.zeros(hd)
+            m.store_f(t.p[5], slice(tile * hd, (tile + 1) * hd), dw, F32)
+
+    # 24, 25, 26: the paged cache (extension)
+    def _paged(self, t):
+        m = self.m
+        d = m.aux_view(t.p[6], 17)
+        T, Hq, Hkv, hd, page, N, B, MP, cdt = d[:9]
+        cu, lens = m.view(t.p[3], I32)[:B + 1], m.view(t.p[4], I32)[:B]
+        table = m.view(t.p[5], I32)[:B * MP].reshape(B, MP)
+        return d, T, Hq, Hkv, hd, page, N, cdt, cu, lens, table
+
+    def _page_rows(self, bid, sid, cdt, shape, at):
+        """[Hkv, hd] f64 values of a pool at (page, slot)."""
+        m = self.m
+        if cdt == I8:
+            q = m.view(bid, I8)[:np.prod(shape)].reshape(shape)[at[0], :, at[1]]
+            s = m.view(sid, F32)[:np.prod(shape[:3])].reshape(shape[:3])[at[0], :, at[1]]
+            return (q.astype(np.float32) * s[:, None]).astype(np.float64)
+        N, H, P, hd = shape
+        idx = ((at[0] * H + np.arange(H)) * P + at[1])[:, None] * hd + np.arange(hd)
+        raw = m.view(bid, cdt)[idx]
+        return (bf16_to_f32(raw) if cdt == BF16 else raw).astype(np.float64)
+
+    def top24(self, t, lo, hi):
+        m = self.m
+        d, T, Hq, Hkv, hd, page, N, cdt, cu, lens, table = self._paged(t)
+        tb = t.p[7] & 0xFF
+        rows = [self._rows3(t.a, t.adt, d[9:12], T, Hkv, hd), self._rows3(t.b, t.adt, d[12:15], T, Hkv, hd)]
+        for r, s, p in paged_rows(T, cu, lens, table, N, page):
+            at = paged_place(table, s, p, N, page)
+            if at is None or not lo * tb <= r < hi * tb:
+                continue
+            for x, bid, sid in ((rows[0], t.dst, t.p[1]), (rows[1], t.p[0], t.p[2])):
+                for h in range(Hkv):
+                    e = (at[0] * Hkv + h) * page + at[1]
+                    if cdt == I8:
+                        q, sc = quantise_row(x[r, h])
+                        m.view(bid, I8)[e * hd:(e + 1) * hd] = q
+                        m.view(sid, F32)[e] = sc
+                    else:
+                        m.store_f(bid, slice(e * hd, (e + 1) * hd), x[r, h], cdt)
+
+    def top25(self, t, lo, hi):
+        m = self.m
+        d, T, Hq, Hkv, hd, page, N, cdt, cu, lens, table = self._paged(t)
+        tb = t.p[7] & 0xFF
+        a, b = lo * tb, min(T, hi * tb)
+        for src, sid, dst in ((t.a, t.p[1], t.dst), (t.b, t.p[2], t.p[0])):
+            out = np.zeros((T, Hkv, hd))
+            for r, s, p in paged_rows(T, cu, lens, table, N, page):
+                at = paged_place(table, s, p, N, page)
+                if at is not None and a <= r < b:
+                    out[r] = self._page_rows(src, sid, cdt, (N, Hkv, page, hd), at)
+            m.store_f(dst, slice(a * Hkv * hd, b * Hkv * hd), out[a:b].reshape(-1), t.dt)
+
+    def top26(self, t, lo, hi):
+        # the workers divide the whole step by its lengths: worker 0 stands for all
+        if lo > 0:
+            return
+        m = self.m
+        d, T, Hq, Hkv, hd, page, N, cdt, cu, lens, table = self._paged(t)
+        shape = (N, Hkv, page, hd)
+
+        def kv(pg, slot):
+            return (self._page_rows(t.b, t.p[1], cdt, shape, (pg, slot)),
+                    self._page_rows(t.p[0], t.p[2], cdt, shape, (pg, slot)))
+        o = paged_attention(self._rows3(t.a, t.adt, d[9:12], T, Hq, hd), kv, cu, lens, table, N, page,
+                            float(_bits_f32(d[15] & 0xFFFFFFFF)), d[16])
+        m.store_f(t.dst, slice(0, T * Hq * hd), o.reshape(-1), t.dt)
+
     # 15: strided partial-axis reduce
     def top15(self, t, lo, hi):
         n_out, red, inner, kind = t.p[0], t.p[1], t.p[2], t.p[3]
@@ -1173,6 +1401,14 @@ def _instr_task(prog: Prog, ins, ew_ts: int, mma_t: int):
     elif op == 68:
         hd, kb, vb, posb, sbits = prog.aux[aux:aux + 5]
         top, p = 21, [imm2, kb, vb, posb, n, hd, imm, sbits]
+    elif op == 69:
+        top, p = 22, [imm2, prog.aux[aux + 13], aux, 1, n, 0, 0, 0]
+    elif op == 70:
+        freq, weight, part, workers = prog.aux[aux + 13:aux + 17]
+        top, p = 23, [imm2, freq, aux, workers, weight, part, 0, 0]
+    elif op in (71, 72, 73):
+        top = 24 + op - 71
+        p = list(prog.aux[aux + 17:aux + 23]) + [aux, n << 8 | 64 if op < 73 else 1]
     elif op == 27:
         M, N, K, G = n, imm >> 16, imm & 0xFFFF, max(1, imm2)
         views = prog.aux[aux:aux + 4] if aux else [0, 0, 0, 0]
@@ -1210,6 +1446,14 @@ def _whole_tiles(t: Task, ew_ts: int, mma_t: int) -> int:
         return max(1, p[3]) * -(-p[1] // p[4])
     if t.top == 21:
         return max(1, (p[4] & 0xFFFF) * max(1, p[4] >> 16))
+    if t.top == 22:
+        return max(1, -(-p[4] * p[3] // 4))
+    if t.top == 23:
+        return max(1, p[3])
+    if t.top in (24, 25):
+        return max(1, -(-(p[7] >> 8) // (p[7] & 0xFF)))
+    if t.top == 26:
+        return max(1, p[7])
     raise NotImplementedError(t.top)
 
 
@@ -1303,6 +1547,7 @@ def execute_schedule(data_or_prog, args, ew_ts: int = 4096, mma_t: int = 128,
             by_lane.setdefault(lane, []).append(e)
         order = list(by_lane)
         base = m.arena.copy()
+        held = {b: a.copy() for b, a in m.ext.items()}      # state buffers, restored like the arena
 
         def go(lanes):
             # each lane runs its entries in stream order; with completion flags
@@ -1310,6 +1555,8 @@ def execute_schedule(data_or_prog, args, ew_ts: int = 4096, mma_t: int = 128,
             # signaled in this phase, so lanes take turns, in `lanes` order,
             # each going as far as it can
             m.arena[:] = base
+            for b, a in held.items():
+                m.ext[b][:] = a
             pos = dict.fromkeys(lanes, 0)
             signaled = set()
             while True:
@@ -1326,7 +1573,7 @@ def execute_schedule(data_or_prog, args, ew_ts: int = 4096, mma_t: int = 128,
                         pos[ln] += 1
                         moved = True
                 if all(pos[ln] == len(by_lane[ln]) for ln in lanes):
-                    return m.arena.copy()
+                    return np.concatenate([m.arena] + [m.ext[b] for b in sorted(m.ext)])
                 if not moved:
                     raise AssertionError("completion flags: a wait that no entry of its phase signals")
 
@@ -1335,7 +1582,11 @@ def execute_schedule(data_or_prog, args, ew_ts: int = 4096, mma_t: int = 128,
             rev = go(order[::-1])
             if not np.array_equal(fwd, rev):
                 raise AssertionError("phase is lane-order dependent (cross-lane race)")
-        m.arena[:] = fwd
+        at = len(m.arena)
+        m.arena[:] = fwd[:at]
+        for b in sorted(m.ext):
+            m.ext[b][:] = fwd[at:at + len(m.ext[b])]
+            at += len(m.ext[b])
 
     n = prog.n_lanes
     streams = prog.streams

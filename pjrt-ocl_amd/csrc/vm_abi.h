@@ -11,7 +11,9 @@ namespace vm {
 // ---- element types (lowering.py:59-81) ------------------------------------------
 enum Dtype : uint32_t {
   DT_F32 = 0, DT_I32 = 1, DT_U32 = 2, DT_BOOL = 3,
-  DT_I64 = 4, DT_F64 = 5, DT_F16 = 6, DT_BF16 = 7, DT_COUNT = 8
+  DT_I64 = 4, DT_F64 = 5, DT_F16 = 6, DT_BF16 = 7,
+  DT_I8 = 8,      // extension: pages of a paged cache only
+  DT_COUNT = 9
 };
 
 // ---- tile ops (scheduler.py:47-71) -----------------------------------------------
@@ -26,7 +28,9 @@ enum TileOp : uint32_t {
   TOP_ARGMAX_SEG = 19,
   TOP_GEMV = 20,
   TOP_DECODE_ATTN = 21,
-  TOP_COUNT = 22
+  TOP_ROTARY = 22, TOP_ROTARY_GRAD = 23,
+  TOP_CACHE_APPEND = 24, TOP_CACHE_READ = 25, TOP_PAGED_ATTN = 26,
+  TOP_COUNT = 27
 };
 
 // ---- elementwise subops (vm_common.cl:118-146) -----------------------------------
@@ -46,6 +50,31 @@ enum EwSub : uint32_t {
 
 // LAYERNORM_SEG p3 flags (extension; 0 = the reference's one-pass core op)
 enum : uint32_t { LN_AFFINE = 1, LN_GELU = 2, LN_TWO_PASS = 4 };
+
+// TOP_ROTARY / TOP_ROTARY_GRAD descriptor flags (aux word RD_FLAGS)
+enum : uint32_t { ROT_INTERLEAVED = 1, ROT_NORM = 2, ROT_INVERSE = 4 };
+// TOP_ROTARY[_GRAD] descriptor (aux words at p2): rows, heads, head size, rotated
+// channels, flags, eps and magnitude bits, then {row stride, head stride, offset} in
+// elements of operand a, and of b for the gradient
+enum : uint32_t {
+  RD_T = 0, RD_H, RD_HD, RD_ROT, RD_FLAGS, RD_EPS, RD_MAG, RD_ARS, RD_AHS, RD_AOFF, RD_BRS, RD_BHS, RD_BOFF, RD_WORDS
+};
+// Descriptor of the paged cache ops (aux words at p6): rows, query heads (the kv heads for
+// append and read), kv heads, head size, positions per page, pages, sequences, pages per
+// table row, the cache's dtype, {row stride, head stride, offset} of operands a and b in
+// elements, scale bits, window (0: none)
+enum : uint32_t {
+  PD_T = 0, PD_HQ, PD_HKV, PD_HD, PD_PAGE, PD_PAGES, PD_SEQS, PD_MAXP, PD_CDT, PD_ARS, PD_AHS, PD_AOFF, PD_BRS,
+  PD_BHS, PD_BOFF, PD_SCALE, PD_WINDOW, PD_WORDS
+};
+// Query heads per kv head, head size, rows per worker's partial block of TOP_PAGED_ATTN at most.
+constexpr uint32_t kPagedMaxGroup = 128;
+constexpr uint32_t kPagedMaxHd = 256;
+constexpr uint32_t kPagedMaxRows = 256;
+
+// A buffer entry whose pad word is BUF_STATE (extension): caller-owned memory bound as a
+// port and written in place; it takes no arena bytes (its offset is past them).
+constexpr uint32_t BUF_STATE = 1;
 
 // ---- entry sentinels (scheduler.py:80-85) -----------------------------------------
 constexpr uint32_t ENT_NOP = 0xFFFFFFFFu;

@@ -138,7 +138,7 @@ VM_DEV uint16_t f32_to_f16(float f) { return __builtin_bit_cast(uint16_t, static
 
 // Element size in bytes of a dtype.
 VM_DEV uint32_t dt_size(uint32_t dt) {
-  return (dt == DT_I64 || dt == DT_F64) ? 8u : dt == DT_BOOL ? 1u
+  return (dt == DT_I64 || dt == DT_F64) ? 8u : (dt == DT_BOOL || dt == DT_I8) ? 1u
        : (dt == DT_F16 || dt == DT_BF16) ? 2u : 4u;
 }
 

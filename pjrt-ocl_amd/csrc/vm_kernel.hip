@@ -15,12 +15,15 @@
 #include <hip/hip_runtime.h>
 
 #include "tile_attn.h"
+#include "tile_cache.h"
 #include "tile_decode.h"
 #include "tile_ew.h"
 #include "tile_gemv.h"
 #include "tile_index.h"
 #include "tile_mma.h"
+#include "tile_paged.h"
 #include "tile_reduce.h"
+#include "tile_rotary.h"
 
 namespace vm {
 
@@ -54,6 +57,11 @@ VM_DEV void exec_tiles(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
     case TOP_ARGMAX_SEG: argmax_tiles(A, ti, lo, hi); break;
     case TOP_GEMV: gemv_tiles(A, ti, lo, hi); break;
     case TOP_DECODE_ATTN: decode_attn_tiles(A, ti, lo, hi); break;
+    case TOP_ROTARY: rotary_tiles(A, ti, lo, hi, false); break;
+    case TOP_ROTARY_GRAD: rotary_tiles(A, ti, lo, hi, true); break;
+    case TOP_CACHE_APPEND: cache_tiles(A, ti, lo, hi, false); break;
+    case TOP_CACHE_READ: cache_tiles(A, ti, lo, hi, true); break;
+    case TOP_PAGED_ATTN: paged_tiles(A, ti, lo, hi); break;
     default: raise_error(A, VM_ERR_BAD_TASK, task_of(A, ti).tile_op); break;
   }
 }

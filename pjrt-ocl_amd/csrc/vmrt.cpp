@@ -68,7 +68,7 @@ std::string hip_msg(hipError_t e) { return std::string(hipGetErrorName(e)) + ": 
 uint32_t dt_size(uint32_t dt) {
   switch (dt) {
     case DT_I64: case DT_F64: return 8;
-    case DT_BOOL: return 1;
+    case DT_BOOL: case DT_I8: return 1;
     case DT_F16: case DT_BF16: return 2;
     default: return 4;
   }
@@ -78,6 +78,7 @@ uint32_t dt_size(uint32_t dt) {
 struct Buffer {
   uint64_t off, size;
   uint32_t dtype;
+  bool state;        // extension: an input written in place, bound as a port (vm_abi.h BUF_STATE)
 };
 struct Program {
   uint64_t arena_bytes = 0;
@@ -136,9 +137,12 @@ bool parse_program(const uint8_t* data, size_t len, Program* P, std::string* err
     b.size = r.get<uint64_t>();
     b.dtype = r.get<uint32_t>();
     const uint32_t pad = r.get<uint32_t>();
-    if (b.off % 64 || b.off + b.size > arena || b.size > arena) return fail(fmt("buffer %u outside arena", i));
+    if (pad != 0 && pad != BUF_STATE) return fail(fmt("buffer %u pad nonzero", i));
+    b.state = pad == BUF_STATE;
+    if (b.state ? (b.off % 64 || b.off < arena || b.size >= (uint64_t(1) << 47))
+                : (b.off % 64 || b.off + b.size > arena || b.size > arena))
+      return fail(fmt("buffer %u outside arena", i));
     if (b.dtype >= DT_COUNT) return fail(fmt("buffer %u dtype %u", i, b.dtype));
-    if (pad) return fail(fmt("buffer %u pad nonzero", i));
     P->buffers.push_back(b);
   }
   auto ids = [&](uint32_t count, std::vector<uint32_t>* out, const char* what) {
@@ -152,6 +156,10 @@ bool parse_program(const uint8_t* data, size_t len, Program* P, std::string* err
     return true;
   };
   if (!ids(n_inputs, &P->inputs, "input") || !ids(n_outputs, &P->outputs, "output")) return false;
+  for (uint32_t i = 0; i < n_buffers; ++i)
+    if (P->buffers[i].state && (std::count(P->inputs.begin(), P->inputs.end(), i) != 1 ||
+                                std::count(P->outputs.begin(), P->outputs.end(), i) != 0))
+      return fail(fmt("state buffer %u is not an input of its own", i));
   auto shape = [&](std::vector<uint64_t>* dims) {
     if (!r.need(8)) return fail("truncated io shape");
     const uint32_t rank = r.get<uint32_t>(), pad = r.get<uint32_t>();
@@ -400,8 +408,91 @@ struct Checker {
       case TOP_FLASH_ATTN: return std::max<uint64_t>(1, uint64_t(t.p[1]) * (cdiv(t.p[2], 256) * 256));   // rows padded to 256-row blocks
       case TOP_GEMV: return t.p[4] ? std::max<uint64_t>(1, t.p[3]) * cdiv(t.p[1], t.p[4]) : 0;
       case TOP_DECODE_ATTN: return std::max<uint64_t>(1, uint64_t(t.p[4] & 0xFFFF) * std::max<uint32_t>(1, t.p[4] >> 16));
+      case TOP_ROTARY: return std::max<uint64_t>(1, cdiv(uint64_t(t.p[4]) * t.p[3], 4));
+      case TOP_ROTARY_GRAD: return std::max<uint32_t>(1, t.p[3]);
+      case TOP_CACHE_APPEND: case TOP_CACHE_READ:
+        return t.p[7] & 0xFF ? std::max<uint64_t>(1, cdiv(t.p[7] >> 8, t.p[7] & 0xFF)) : 0;
+      case TOP_PAGED_ATTN: return std::max<uint32_t>(1, t.p[7]);
       default: return 0;
     }
+  }
+
+  // [T, H, hd] rows of buffer `id` at aux words {row stride, head stride, offset}
+  bool rows_ok(uint32_t id, uint32_t dt, const int32_t* st, uint64_t T, uint64_t H, uint64_t hd) const {
+    for (int k = 0; k < 3; ++k)
+      if (st[k] < 0) return false;
+    const uint64_t last = uint64_t(st[2]) + (T - 1) * uint64_t(st[0]) + (H - 1) * uint64_t(st[1]) + hd - 1;
+    return id < P.buffers.size() && last < elems(id, dt);
+  }
+
+  // Rotary positions and the paged cache (extensions)
+  bool check_serving(uint32_t ti) {
+    const Task& t = P.tasks[ti];
+    const uint32_t top = t.tile_op & 0xFF, dt = (t.tile_op >> 8) & 0xFF, adt = (t.tile_op >> 16) & 0xFF;
+    const uint32_t nb = uint32_t(P.buffers.size());
+    auto has = [&](uint32_t id, uint64_t n, uint32_t d) { return id < nb && elems(id, d) >= n; };
+    auto flt = [](uint32_t d) { return d == DT_F32 || d == DT_F16 || d == DT_BF16; };
+    if (top == TOP_ROTARY || top == TOP_ROTARY_GRAD) {
+      if (!aux_ok(t.p[2], RD_WORDS)) return fail(ti, "rotary descriptor");
+      const int32_t* d = P.aux.data() + t.p[2];
+      const int64_t T = d[RD_T], H = d[RD_H], hd = d[RD_HD], rot = d[RD_ROT];
+      if (dt != adt || !flt(dt)) return fail(ti, "rotary dtype");
+      if (T < 1 || H < 1 || H > (1 << 16) || hd < 2 || hd > 256 || hd % 2 || rot < 2 || rot > hd || rot % 2 ||
+          uint32_t(d[RD_FLAGS]) > (ROT_INTERLEAVED | ROT_NORM | ROT_INVERSE) || uint64_t(T) * H > 0x7FFFFFFFull)
+        return fail(ti, "rotary shape");
+      if (!has(t.p[0], T, DT_I32) || !has(t.p[1], rot, DT_U32)) return fail(ti, "rotary positions / frequencies");
+      if (!rows_ok(t.a, adt, d + RD_ARS, T, H, hd)) return fail(ti, "rotary rows");
+      if (!has(t.dst, uint64_t(T) * H * hd, dt)) return fail(ti, "rotary result");
+      if (top == TOP_ROTARY) {
+        if (t.p[3] < 1 || t.p[3] > uint32_t(H) || t.p[4] != uint32_t(T)) return fail(ti, "rotary splits");
+        return !(d[RD_FLAGS] & ROT_NORM) || has(t.b, hd, DT_F32) || fail(ti, "rotary weight");
+      }
+      if (t.p[3] < 1 || t.p[3] > 4096) return fail(ti, "rotary gradient workers");
+      if (!rows_ok(t.b, adt, d + RD_BRS, T, H, hd)) return fail(ti, "rotary gradient's rows");
+      return (has(t.p[4], hd, DT_F32) && has(t.p[5], uint64_t(t.p[3]) * hd, DT_F32)) ||
+             fail(ti, "rotary gradient's weight");
+    }
+    if (!aux_ok(t.p[6], PD_WORDS)) return fail(ti, "paged cache descriptor");
+    const int32_t* d = P.aux.data() + t.p[6];
+    const int64_t T = d[PD_T], Hq = d[PD_HQ], Hkv = d[PD_HKV], hd = d[PD_HD], page = d[PD_PAGE], N = d[PD_PAGES],
+                  B = d[PD_SEQS], MP = d[PD_MAXP];
+    const uint32_t cdt = uint32_t(d[PD_CDT]);
+    if (T < 1 || T >= (1 << 24) || Hkv < 1 || Hkv > (1 << 16) || hd < 8 || hd % 8 || hd > kPagedMaxHd || page < 1 ||
+        page > (1 << 16) || N < 1 || B < 1 || MP < 1 || B * MP >= (int64_t(1) << 31) || MP * page >= (int64_t(1) << 31) ||
+        N * Hkv * page >= (int64_t(1) << 40))
+      return fail(ti, "paged cache shape");
+    if (!flt(cdt) && cdt != DT_I8) return fail(ti, "paged cache dtype");
+    // the pages: a, b of read, dst, p0 of append, b, p0 of attention
+    const uint32_t kp = top == TOP_CACHE_READ ? t.a : top == TOP_CACHE_APPEND ? t.dst : t.b;
+    const uint32_t vp = top == TOP_CACHE_READ ? t.b : t.p[0];
+    const uint64_t slots = uint64_t(N) * Hkv * page;
+    for (uint32_t id : {kp, vp})
+      if (!has(id, slots * hd, cdt) || P.buffers[id].dtype != cdt) return fail(ti, "paged cache pages");
+    if (cdt == DT_I8 && (!has(t.p[1], slots, DT_F32) || !has(t.p[2], slots, DT_F32))) return fail(ti, "paged cache scales");
+    if (!has(t.p[1], 0, DT_F32) || !has(t.p[2], 0, DT_F32)) return fail(ti, "paged cache scales");
+    if (!has(t.p[3], B + 1, DT_I32) || !has(t.p[4], B, DT_I32) || !has(t.p[5], uint64_t(B) * MP, DT_I32))
+      return fail(ti, "paged cache batch");
+    if (top == TOP_PAGED_ATTN) {
+      if (dt != adt || !flt(dt) || (cdt != dt && cdt != DT_I8)) return fail(ti, "paged attention dtype");
+      if (Hq < 1 || Hq % Hkv || Hq / Hkv > kPagedMaxGroup || d[PD_WINDOW] < 0) return fail(ti, "paged attention shape");
+      if (t.p[7] < 1 || t.p[7] > kMaxLanes) return fail(ti, "paged attention workers");
+      if (!rows_ok(t.a, adt, d + PD_ARS, T, Hq, hd)) return fail(ti, "paged attention queries");
+      return has(t.dst, uint64_t(T) * Hq * hd, dt) || fail(ti, "paged attention output");
+    }
+    const uint32_t tb = t.p[7] & 0xFF;
+    if (tb < 1 || tb > 64 || t.p[7] >> 8 != uint32_t(T)) return fail(ti, "paged cache rows per tile");
+    if (top == TOP_CACHE_READ) {
+      if (!flt(dt) || adt != cdt) return fail(ti, "cache read dtype");
+      return (has(t.dst, uint64_t(T) * Hkv * hd, dt) && has(t.p[0], uint64_t(T) * Hkv * hd, dt)) ||
+             fail(ti, "cache read rows");
+    }
+    if (top != TOP_CACHE_APPEND) return fail(ti, fmt("tile op %u is not supported by this runtime", top));
+    if (!flt(adt) || dt != cdt || (cdt != adt && cdt != DT_I8)) return fail(ti, "cache append dtype");
+    if (!P.buffers[kp].state || !P.buffers[vp].state ||
+        (cdt == DT_I8 && (!P.buffers[t.p[1]].state || !P.buffers[t.p[2]].state)))
+      return fail(ti, "cache append writes state buffers");
+    return (rows_ok(t.a, adt, d + PD_ARS, T, Hkv, hd) && rows_ok(t.b, adt, d + PD_BRS, T, Hkv, hd)) ||
+           fail(ti, "cache append rows");
   }
 
   bool check(uint32_t ti) {
@@ -409,6 +500,8 @@ struct Checker {
     const uint32_t top = t.tile_op & 0xFF, dt = (t.tile_op >> 8) & 0xFF, adt = (t.tile_op >> 16) & 0xFF;
     const uint32_t nb = uint32_t(P.buffers.size());
     auto has = [&](uint32_t id, uint64_t n, uint32_t d) { return id < nb && elems(id, d) >= n; };
+    if (top >= TOP_ROTARY) return check_serving(ti);
+    if (dt == DT_I8 || adt == DT_I8) return fail(ti, "i8 is the element type of a paged cache only");
     switch (top) {
       case TOP_EW: {
         const uint32_t sub = t.p[0];
@@ -751,7 +844,8 @@ struct vmrt_program {
   uint32_t launch_seq = 0;                    // launches so far (completion flag values)
   uint32_t* task_scratch = nullptr;           // per task: byte offset of its scratch region
   std::vector<int> input_port, output_port;   // -1 = arena copy
-  std::vector<uint32_t> in_bytes, out_bytes;
+  std::vector<uint64_t> in_bytes, out_bytes;
+  std::vector<uint32_t> states;               // inputs written in place
   hipStream_t last_stream = nullptr;          // the stream of the latest launch (null: none yet)
   bool launched = false;
   VmArgs args{};
@@ -1087,8 +1181,8 @@ static int prepare_program(vmrt_runtime* rt, vmrt_program* lp, const void* bytes
                        rt->info.max_lanes));
 
   // control uniformity across lanes, then the completion flags
+  std::vector<CtlSig> sigs(n_lanes);
   {
-    std::vector<CtlSig> sigs(n_lanes);
     for (uint32_t l = 0; l < n_lanes; ++l) {
       CtlSig& s = sigs[l];
       if (!control_sig(P, l, 0, P.lanes[l].root_len, 0, &s, &msg))
@@ -1133,6 +1227,9 @@ static int prepare_program(vmrt_runtime* rt, vmrt_program* lp, const void* bytes
     if (next_port >= kMaxPorts) return -1;
     return port_of[id] = next_port++;
   };
+  for (uint32_t id : P.inputs)          // state buffers have no other place than a port
+    if (P.buffers[id].state && assign(id) < 0)
+      return set_err(err, errlen, VMRT_INVALID_ARGUMENT, fmt("LoadedProgram: more than %d state buffers", kMaxPorts));
   for (uint32_t id : P.inputs) lp->input_port.push_back(assign(id));
   for (uint32_t id : P.outputs) lp->output_port.push_back(assign(id));
   // a constant buffer is arena-resident; a port never aliases one
@@ -1165,6 +1262,12 @@ static int prepare_program(vmrt_runtime* rt, vmrt_program* lp, const void* bytes
     if (top == TOP_GEMV && orig.p[6]) t.p[7] = handle(orig.p[7]);
     if (top == TOP_DECODE_ATTN)
       for (int k = 0; k < 4; ++k) t.p[k] = handle(orig.p[k]);
+    if (top == TOP_ROTARY || top == TOP_ROTARY_GRAD)
+      for (int k = 0; k < 2; ++k) t.p[k] = handle(orig.p[k]);
+    if (top == TOP_ROTARY_GRAD)
+      for (int k = 4; k < 6; ++k) t.p[k] = handle(orig.p[k]);
+    if (top == TOP_CACHE_APPEND || top == TOP_CACHE_READ || top == TOP_PAGED_ATTN)
+      for (int k = 0; k < 6; ++k) t.p[k] = handle(orig.p[k]);
   }
   // ---- patch aux: runtime start-scalar / index-buffer locations (runtime.cc:883-924) ----
   std::vector<int32_t>& aux = pr->aux;
@@ -1220,13 +1323,44 @@ static int prepare_program(vmrt_runtime* rt, vmrt_program* lp, const void* bytes
     if (lp->scratch_bytes > 0xFFFFFFFFull)
       return set_err(err, errlen, VMRT_RESOURCE_EXHAUSTED, "LoadedProgram: task scratch exceeds 4 GiB");
   }
+  // Paged attention's partials are megabytes per task, so tasks that never run between
+  // the same pair of grid barriers (a decoder's layers) share a region; the arrival
+  // counters in it are zero again when a task ends.
+  {
+    std::map<uint32_t, std::set<uint64_t>> segs;
+    uint64_t most = 0;
+    for (uint32_t l = 0; l < n_lanes; ++l)
+      for (const auto& e : sigs[l].tiles) {
+        const uint32_t ti = P.entries[P.lanes[l].off + e.first].task;
+        if ((P.tasks[ti].tile_op & 0xFF) == TOP_PAGED_ATTN) segs[ti].insert(e.second);
+      }
+    for (const auto& kv : segs) most = std::max(most, paged_scratch_bytes(P.tasks[kv.first], P.aux.data()));
+    most = (most + 255) & ~uint64_t(255);
+    std::vector<std::pair<uint32_t, std::set<uint64_t>>> regions;      // offset, segments in use
+    for (const auto& kv : segs) {
+      auto free = [&](const std::set<uint64_t>& used) {
+        return std::none_of(kv.second.begin(), kv.second.end(), [&](uint64_t s) { return used.count(s) != 0; });
+      };
+      auto it = std::find_if(regions.begin(), regions.end(), [&](const auto& r) { return free(r.second); });
+      if (it == regions.end()) {
+        if (lp->scratch_bytes + most > 0xFFFFFFFFull)
+          return set_err(err, errlen, VMRT_RESOURCE_EXHAUSTED, "LoadedProgram: task scratch exceeds 4 GiB");
+        it = regions.insert(regions.end(), {uint32_t(lp->scratch_bytes), {}});
+        lp->scratch_bytes += most;
+      }
+      it->second.insert(kv.second.begin(), kv.second.end());
+      task_scratch[kv.first] = it->first;
+    }
+  }
   // completion flags: 64-bit words after the task scratch (zeroed with it)
   lp->flag_off = lp->scratch_bytes;
   lp->scratch_bytes += (uint64_t(P.n_flags) * 8 + 255) & ~uint64_t(255);
   if (lp->scratch_bytes > 0xFFFFFFFFull)
     return set_err(err, errlen, VMRT_RESOURCE_EXHAUSTED, "LoadedProgram: task scratch exceeds 4 GiB");
-  for (size_t i = 0; i < P.inputs.size(); ++i) lp->in_bytes.push_back(uint32_t(P.buffers[P.inputs[i]].size));
-  for (size_t i = 0; i < P.outputs.size(); ++i) lp->out_bytes.push_back(uint32_t(P.buffers[P.outputs[i]].size));
+  for (size_t i = 0; i < P.inputs.size(); ++i) lp->in_bytes.push_back(P.buffers[P.inputs[i]].size);
+  for (size_t i = 0; i < P.outputs.size(); ++i) lp->out_bytes.push_back(P.buffers[P.outputs[i]].size);
+  for (size_t i = 0; i < P.inputs.size(); ++i)
+    if (P.buffers[P.inputs[i]].state) lp->states.push_back(uint32_t(i));
 
   return VMRT_OK;
 }
@@ -1334,6 +1468,21 @@ static int enqueue_locked(vmrt_program* p, const void* const* inputs, size_t n_i
     return set_err(err, errlen, VMRT_INVALID_ARGUMENT,
                    fmt("expected %zu inputs and %zu outputs, got %zu and %zu", P.inputs.size(), P.outputs.size(), n_in,
                        n_out));
+  // state buffers: 16-byte aligned, and no other buffer of the launch on their memory
+  for (uint32_t i : p->states) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(inputs[i]), hi = lo + p->in_bytes[i];
+    if (lo % 16) return set_err(err, errlen, VMRT_INVALID_ARGUMENT, fmt("state input %u is not 16-byte aligned", i));
+    auto meets = [&](const void* q, uint64_t n) {
+      const uintptr_t a0 = reinterpret_cast<uintptr_t>(q);
+      return a0 < hi && lo < a0 + n;
+    };
+    for (size_t k = 0; k < n_in; ++k)
+      if (k != i && meets(inputs[k], p->in_bytes[k]))
+        return set_err(err, errlen, VMRT_INVALID_ARGUMENT, fmt("state input %u overlaps input %zu", i, k));
+    for (size_t k = 0; k < n_out; ++k)
+      if (meets(outputs[k], p->out_bytes[k]))
+        return set_err(err, errlen, VMRT_INVALID_ARGUMENT, fmt("state input %u overlaps output %zu", i, k));
+  }
   VmArgs a = p->args;
   a.seq = ++p->launch_seq;     // a new identity for this launch's completion flag values
   hipError_t e = hipSuccess;

@@ -15,6 +15,7 @@ lowering.py:286-331), so the resulting bytes are a reference-format program.
 from __future__ import annotations
 
 import dataclasses
+import fractions
 import math
 
 import numpy as np
@@ -58,6 +59,81 @@ class GraphError(ValueError):
     pass
 
 
+@dataclasses.dataclass(frozen=True)
+class PagedCache:
+    """Keys and values of many sequences in pages that the caller owns and the
+    program writes in place (``Graph.paged_cache``): pages [N, heads, page, head_dim]
+    of one dtype, or i8 with one f32 scale per (page, head, position)."""
+    k: Tensor
+    v: Tensor
+    k_scale: Tensor | None
+    v_scale: Tensor | None
+
+    @property
+    def dims(self) -> tuple:
+        return self.k.shape
+
+
+@dataclasses.dataclass(frozen=True)
+class PagedBatch:
+    """The rows of a step (``Graph.paged_batch``): sequence s's new tokens are rows
+    cu[s] .. cu[s + 1] - 1, its length with them is lens[s], and position p of it
+    lies in page table[s, p // page]."""
+    cu: Tensor
+    lens: Tensor
+    table: Tensor
+
+
+def rotary_frequencies(rot: int, theta: float = 10000.0, factor: float = 1.0, original: int = 0,
+                       low: float = 1.0, high: float = 32.0) -> np.ndarray:
+    """Radians per position of each of the rot / 2 channel pairs, f64:
+    theta^(-2 i / rot).  ``factor`` > 1 stretches positions for contexts longer than
+    the ``original`` one the model was trained on: frequencies that turn fewer than
+    ``low`` times over it are divided by the factor, those of more than ``high`` turns
+    are kept, and the ones between are blended linearly in their turns;
+    with ``original`` 0 every frequency is divided."""
+    if rot < 2 or rot % 2:
+        raise GraphError("rotary_frequencies: rot is even and at least 2")
+    if not (theta > 0 and factor >= 1.0 and original >= 0 and 0 <= low < high):
+        raise GraphError("rotary_frequencies: theta > 0, factor >= 1, original >= 0 and 0 <= low < high")
+    f = float(theta) ** (-2.0 * np.arange(rot // 2, dtype=np.float64) / rot)
+    if factor == 1.0:
+        return f
+    if not original:
+        return f / factor
+    keep = np.clip((original * f / (2.0 * np.pi) - low) / (high - low), 0.0, 1.0)
+    return f * keep + f / factor * (1.0 - keep)
+
+
+def _two_pi_inverse_2_192() -> int:
+    """floor(2^192 / (2 pi)) by Machin's formula pi = 16 atan(1/5) - 4 atan(1/239)."""
+    one = 1 << 256
+
+    def atan_inv(k):
+        total, power, n = 0, one // k, 1
+        while power:
+            total += power // n if n % 4 == 1 else -(power // n)
+            power //= k * k
+            n += 2
+        return total
+    pi = 16 * atan_inv(5) - 4 * atan_inv(239)          # pi 2^256
+    return (1 << 447) // pi                            # 2^192 / (2 pi)
+
+
+_INV_2PI = fractions.Fraction(_two_pi_inverse_2_192(), 1 << 192)
+
+
+def turn_words(inv_freq) -> np.ndarray:
+    """[R, 2] u32: each frequency (radians per position) as the low and high words of
+    its 64-bit fixed-point fraction of a turn, so that position * frequency modulo one
+    turn is one integer product, exact to 2^-33 turns for every 32-bit position."""
+    out = np.empty((len(inv_freq), 2), np.uint32)
+    for i, f in enumerate(inv_freq):
+        w = round(fractions.Fraction(float(f)) * _INV_2PI * (1 << 64)) & ((1 << 64) - 1)
+        out[i] = (w & 0xFFFFFFFF, w >> 32)
+    return out
+
+
 class Graph:
     def __init__(self):
         self.buffers: list = []         # [(n_elems, dtype)]
@@ -70,6 +146,7 @@ class Graph:
         self._stack: list = []          # instruction lists under construction
         self._disjoint = 0
         self.aliases: dict = {}         # buffer -> (parent buffer, byte offset)
+        self.states: set = set()        # inputs written in place
 
     # ---- buffers / io -----------------------------------------------------
     def _new(self, shape, dtype) -> Tensor:
@@ -80,6 +157,14 @@ class Graph:
     def input(self, shape, dtype="f32") -> Tensor:
         t = self._new(shape, dtype)
         self.inputs.append(t)
+        return t
+
+    def state(self, shape, dtype="f32") -> Tensor:
+        """An input that the program's tasks write in place: memory the caller owns
+        and keeps between runs, such as a cache.  It takes no arena bytes, so it may
+        be of any size, and must not overlap another input or output of the run."""
+        t = self.input(shape, dtype)
+        self.states.add(t.buf)
         return t
 
     def const(self, value, dtype=None) -> Tensor:
@@ -108,6 +193,8 @@ class Graph:
 
     def output(self, *ts: Tensor) -> None:
         for t in ts:
+            if t.buf in self.states:
+                raise GraphError("a state buffer is updated in place and is no output")
             self.outputs.append(t)
 
     def add_aux(self, words) -> int:
@@ -150,6 +237,8 @@ class Graph:
         byte_off = elem_off * V.DT_SIZE[src.dtype]
         if byte_off % 16:
             raise GraphError("alias offset must keep 16-byte alignment")
+        if src.buf in self.states:
+            raise GraphError("alias of a state buffer")
         parent, base = self.aliases.get(src.buf, (src.buf, 0))
         t = self._new(shape, src.dtype)
         self.aliases[t.buf] = (parent, base + byte_off)
@@ -518,6 +607,206 @@ class Graph:
                           reads_hint=(cache_v.buf, k.buf, v.buf, pos.buf)))
         return dst
 
+    # ---- rotary positions and the paged cache (extensions) ------------------------
+    def _heads_view(self, t: Tensor, what: str) -> tuple:
+        """(buffer, row stride, head stride, offset) of [rows, heads, head_dim] rows:
+        a plain tensor, or a view of one whose last stride is 1."""
+        if len(t.shape) != 3:
+            raise GraphError(f"{what}: [rows, heads, head_dim], got {t.shape}")
+        if not t.view:
+            return t.buf, t.shape[1] * t.shape[2], t.shape[2], 0
+        w = self.aux[t.view - 1:t.view - 1 + 8]
+        w = [x - (1 << 32) if x >= 1 << 31 else x for x in w]
+        (rs, hs, cs), off = w[4:7], w[7]
+        if cs != 1 and t.shape[2] > 1 or min(rs, hs, off) < 0:
+            raise GraphError(f"{what}: a view needs contiguous channels and strides of at least 0")
+        return t.buf, rs, hs, off
+
+    def _floats(self, what: str, *ts: Tensor) -> int:
+        dts = {t.dtype for t in ts}
+        if len(dts) != 1 or next(iter(dts)) not in (V.DT_F32, V.DT_F16, V.DT_BF16):
+            raise GraphError(f"{what}: operands share one of f32, f16 and bf16")
+        return next(iter(dts))
+
+    def _rotary_args(self, what, x, pos, inv_freq, weight, eps):
+        T, H, hd = x.shape
+        inv_freq = [float(f) for f in inv_freq]
+        rot = 2 * len(inv_freq)
+        if hd % 2 or not 2 <= hd <= 256 or not 2 <= rot <= hd:
+            raise GraphError(f"{what}: head_dim {hd} is even and at most 256, with 2 .. head_dim rotated channels, not {rot}")
+        if T < 1 or H < 1:
+            raise GraphError(f"{what}: no rows")
+        if not all(math.isfinite(f) for f in inv_freq):
+            raise GraphError(f"{what}: frequencies are finite")
+        if pos.shape != (T,) or pos.dtype != V.DT_I32 or pos.view:
+            raise GraphError(f"{what}: positions are i32 [{T}]")
+        if weight is not None and (weight.shape != (hd,) or weight.dtype != V.DT_F32 or weight.view):
+            raise GraphError(f"{what}: the norm's weight is f32 [{hd}]")
+        if not eps >= 0.0:
+            raise GraphError(f"{what}: eps is at least 0")
+        return rot, self.const(turn_words(inv_freq), "u32")
+
+    def rotary(self, x: Tensor, pos: Tensor, inv_freq, weight: Tensor | None = None, eps: float = 1e-6,
+               interleaved: bool = False, magnitude: float = 1.0, inverse: bool = False) -> Tensor:
+        """Rotary positions of the heads of x [T, H, hd], a tensor or a view of a wider
+        row (queries inside a fused projection): channel pair i of row t is rotated by
+        pos[t] * inv_freq[i] radians and scaled by ``magnitude``, channels past the
+        2 len(inv_freq) rotated ones pass.  Pairs are (i, i + R) of R = len(inv_freq), or
+        (2 i, 2 i + 1) with ``interleaved``.  With ``weight`` (f32 [hd]) each head is
+        first normalised: x / sqrt(mean(x^2) + eps) * weight, in the same pass.
+        ``inverse`` rotates back, which is the gradient of the rotation without a
+        norm.  Angles are exact to 2^-32 turns at every 32-bit position; arithmetic is
+        f32, rounded once.  Returns [T, H, hd] of x's dtype."""
+        what = "rotary"
+        buf, rs, hs, off = self._heads_view(x, what)
+        dt = self._floats(what, x)
+        rot, freq = self._rotary_args(what, x, pos, inv_freq, weight, eps)
+        T, H, hd = x.shape
+        flags = interleaved * V.ROT_INTERLEAVED | (weight is not None) * V.ROT_NORM | inverse * V.ROT_INVERSE
+        desc = self.add_aux([T, H, hd, rot, flags, V.f32_bits(eps), V.f32_bits(magnitude), rs, hs, off, 0, 0, 0,
+                             freq.buf])
+        dst = self._new(x.shape, dt)
+        wb = weight.buf if weight is not None else buf
+        self.emit(V.Instr(V.OP_ROTARY, dst=dst.buf, a=buf, b=wb, n=T, imm=H, aux=desc, imm2=pos.buf,
+                          reads_hint=(pos.buf, freq.buf)))
+        return dst
+
+    def rotary_grad(self, dy: Tensor, x: Tensor, pos: Tensor, inv_freq, weight: Tensor | None = None,
+                    eps: float = 1e-6, interleaved: bool = False, magnitude: float = 1.0):
+        """Gradients of ``rotary`` at x: (dx of x's dtype, dweight f32 [hd], or None
+        without a norm).  Sums over rows are f32, in an order that depends on the
+        shapes alone."""
+        what = "rotary_grad"
+        if dy.shape != x.shape:
+            raise GraphError(f"{what}: dy {dy.shape} and x {x.shape}")
+        dt = self._floats(what, dy, x)
+        if weight is None:
+            return self.rotary(dy, pos, inv_freq, interleaved=interleaved, magnitude=magnitude, inverse=True), None
+        (db, drs, dhs, doff), (xb, xrs, xhs, xoff) = self._heads_view(dy, what), self._heads_view(x, what)
+        rot, freq = self._rotary_args(what, x, pos, inv_freq, weight, eps)
+        T, H, hd = x.shape
+        flags = interleaved * V.ROT_INTERLEAVED | V.ROT_NORM
+        dst = self._new(x.shape, dt)
+        workers = rotary_grad_workers(T, H)
+        part = self._new((workers, hd), V.DT_F32)
+        desc = self.add_aux([T, H, hd, rot, flags, V.f32_bits(eps), V.f32_bits(magnitude), drs, dhs, doff,
+                             xrs, xhs, xoff, freq.buf, weight.buf, part.buf, workers])
+        self.emit(V.Instr(V.OP_ROTARY_GRAD, dst=dst.buf, a=db, b=xb, n=T, imm=H, aux=desc, imm2=pos.buf,
+                          reads_hint=(pos.buf, freq.buf, weight.buf)))
+        return dst, self.reduce_axis(part, 0, V.RED_SUM)
+
+    def paged_cache(self, pages: int, heads: int, page: int, head_dim: int, dtype="bf16") -> PagedCache:
+        """State inputs of a cache of ``pages`` pages of ``page`` positions: k and v
+        pages [pages, heads, page, head_dim], and for i8 the scales [pages, heads,
+        page] f32 of k and of v, in this order.  Any page size; head_dim a multiple of
+        8 up to 256."""
+        dt = _dt(dtype)
+        if dt not in (V.DT_F32, V.DT_F16, V.DT_BF16, V.DT_I8):
+            raise GraphError("paged_cache: pages are f32, f16, bf16 or i8")
+        if pages < 1 or heads < 1 or page < 1 or head_dim % 8 or not 8 <= head_dim <= 256:
+            raise GraphError("paged_cache: at least one page, head and position; head_dim a multiple of 8 up to 256")
+        if page > 1 << 16 or pages >= 1 << 31 or heads > 1 << 16 or pages * heads * page >= 1 << 40:
+            raise GraphError("paged_cache: too large")
+        shape = (pages, heads, page, head_dim)
+        k, v = self.state(shape, dt), self.state(shape, dt)
+        ks = vs = None
+        if dt == V.DT_I8:
+            ks, vs = self.state(shape[:3], "f32"), self.state(shape[:3], "f32")
+        return PagedCache(k, v, ks, vs)
+
+    def paged_batch(self, seqs: int, max_pages: int) -> PagedBatch:
+        """i32 inputs that describe the rows of a step, in this order: cu [seqs + 1],
+        lens [seqs], table [seqs, max_pages] (see ``PagedBatch``).  They are read on
+        the device, so one program serves every batch of the same shape: unused
+        sequences have no rows, and rows past cu[seqs] belong to no sequence."""
+        if seqs < 1 or max_pages < 1 or seqs * max_pages >= 1 << 31:
+            raise GraphError("paged_batch: at least one sequence and page")
+        return PagedBatch(self.input((seqs + 1,), "i32"), self.input((seqs,), "i32"),
+                          self.input((seqs, max_pages), "i32"))
+
+    def _paged(self, what, cache, batch, T, Hq, a, b, scale=0.0, window=0):
+        """Descriptor words of a paged cache op (vm_abi.h ``PD_*``) with its operands'
+        strides, and the buffers of the cache and the batch that follow it."""
+        N, Hkv, P, hd = cache.dims
+        B, MP = batch.table.shape
+        if batch.cu.shape != (B + 1,) or batch.lens.shape != (B,):
+            raise GraphError(f"{what}: cu is [seqs + 1] and lens [seqs] of the table's seqs")
+        for t in (batch.cu, batch.lens, batch.table):
+            if t.dtype != V.DT_I32 or t.view:
+                raise GraphError(f"{what}: cu, lens and table are i32")
+        if MP * P >= 1 << 31:
+            raise GraphError(f"{what}: positions of a sequence fit 31 bits")
+        ks = cache.k_scale.buf if cache.k_scale is not None else cache.k.buf
+        vs = cache.v_scale.buf if cache.v_scale is not None else cache.v.buf
+        return [T, Hq, Hkv, hd, P, N, B, MP, cache.k.dtype, *a, *b, V.f32_bits(scale), window], \
+            [ks, vs, batch.cu.buf, batch.lens.buf, batch.table.buf]
+
+    def cache_append(self, cache: PagedCache, batch: PagedBatch, k: Tensor, v: Tensor) -> None:
+        """Write the new rows' keys and values, [T, heads, head_dim] (tensors or views
+        of wider rows), into the cache's pages in place: row r of sequence s is
+        position lens[s] - (cu[s + 1] - r).  Pages of i8 take rint(x / scale) of each
+        row's scale = max|x| / 127, both f32 (a row of zeros: scale 0; one with an
+        infinity or NaN: scale NaN).  Not written: rows of no sequence, sequences whose
+        length is less than their new rows or more than the table's pages hold, and
+        positions whose table entry is no page (any number outside [0, N)).  Two
+        sequences' new rows must not share a position of a page."""
+        what = "cache_append"
+        dt = self._floats(what, k, v)
+        if k.shape != v.shape or len(k.shape) != 3 or k.shape[1:] != (cache.dims[1], cache.dims[3]):
+            raise GraphError(f"{what}: k and v are [rows, {cache.dims[1]}, {cache.dims[3]}], not {k.shape} and {v.shape}")
+        if cache.k.dtype not in (dt, V.DT_I8):
+            raise GraphError(f"{what}: rows of {V.DT_NAMES[dt]} into pages of {V.DT_NAMES[cache.k.dtype]}")
+        if k.shape[0] < 1:
+            raise GraphError(f"{what}: no rows")
+        (kb, *ka), (vb, *va) = self._heads_view(k, what), self._heads_view(v, what)
+        words, bufs = self._paged(what, cache, batch, k.shape[0], cache.dims[1], ka, va)
+        desc = self.add_aux(words + [cache.v.buf] + bufs)
+        self.emit(V.Instr(V.OP_CACHE_APPEND, dst=cache.k.buf, a=kb, b=vb, n=k.shape[0], aux=desc))
+
+    def cache_read(self, cache: PagedCache, batch: PagedBatch, rows: int, dtype="f32") -> tuple:
+        """The keys and values that ``cache_append`` of the same batch has its rows
+        at, as two tensors [rows, heads, head_dim]: with cu the sums of lens, whole
+        sequences one after another.  i8 pages give q * scale, rounded once to
+        ``dtype``.  Rows that append would not write are 0."""
+        what = "cache_read"
+        dt = _dt(dtype)
+        if dt not in (V.DT_F32, V.DT_F16, V.DT_BF16) or rows < 1:
+            raise GraphError(f"{what}: at least one row of f32, f16 or bf16")
+        N, Hkv, P, hd = cache.dims
+        words, bufs = self._paged(what, cache, batch, rows, Hkv, (0, 0, 0), (0, 0, 0))
+        k, v = self._new((rows, Hkv, hd), dt), self._new((rows, Hkv, hd), dt)
+        desc = self.add_aux(words + [v.buf] + bufs)
+        self.emit(V.Instr(V.OP_CACHE_READ, dst=k.buf, a=cache.k.buf, b=cache.v.buf, n=rows, aux=desc))
+        return k, v
+
+    def paged_attention(self, q: Tensor, cache: PagedCache, batch: PagedBatch, scale: float,
+                        window: int = 0) -> Tensor:
+        """Causal attention of the new rows' queries q [T, Hq, head_dim] (a tensor or a
+        view of wider rows) over the cache, their own positions included (``cache_append``
+        first): the row at position p of a sequence sees positions p' <= p, with
+        ``window`` > 0 only those above p - window, and query head h reads kv head
+        h // (Hq // heads).  Chunks and single tokens mix freely in one batch.
+        Positions whose table entry is no page are not seen.  Rows that see nothing,
+        rows of no sequence and rows of a sequence whose length is less than its
+        new rows or more than its pages hold are 0.  Sums and softmax are f32.
+        Returns [T, Hq, head_dim] of q's dtype, which is the pages' or any for i8."""
+        what = "paged_attention"
+        dt = self._floats(what, q)
+        N, Hkv, P, hd = cache.dims
+        buf, rs, hs, off = self._heads_view(q, what)
+        T, Hq, qd = q.shape
+        if qd != hd or Hq < 1 or Hq % Hkv or Hq // Hkv > V.PAGED_MAX_GROUP or T < 1:
+            raise GraphError(f"{what}: queries {q.shape} of {Hkv} kv heads of {hd} (at most {V.PAGED_MAX_GROUP} to one)")
+        if cache.k.dtype not in (dt, V.DT_I8):
+            raise GraphError(f"{what}: queries of {V.DT_NAMES[dt]} over pages of {V.DT_NAMES[cache.k.dtype]}")
+        if not (scale > 0 and math.isfinite(scale)) or window < 0 or window >= 1 << 31:
+            raise GraphError(f"{what}: scale > 0 and window >= 0")
+        words, bufs = self._paged(what, cache, batch, T, Hq, (rs, hs, off), (0, 0, 0), scale, window)
+        dst = self._new(q.shape, dt)
+        desc = self.add_aux(words + [cache.v.buf] + bufs)
+        self.emit(V.Instr(V.OP_PAGED_ATTN, dst=dst.buf, a=buf, b=cache.k.buf, n=T, imm=Hq, aux=desc))
+        return dst
+
     # ---- dynamic slices / gathers ------------------------------------------------
     def dynamic_slice(self, a: Tensor, starts, sizes) -> Tensor:
         a = self.materialize(a)
@@ -623,12 +912,16 @@ class Graph:
         bufs, off = [], 0
         for i, (n, dt) in enumerate(self.buffers):
             size = n * V.DT_SIZE[dt]
+            if i in self.states:            # takes no arena bytes: placed past them below
+                bufs.append(V.Buffer(0, size, dt, True))
+                continue
             if i in self.aliases:           # shares its parent's memory
                 parent, byte_off = self.aliases[i]
                 bufs.append(V.Buffer(bufs[parent].arena_byte_offset + byte_off, size, dt))
                 continue
             bufs.append(V.Buffer(off, size, dt))
             off += max(ARENA_SLOT, -(-size // V.ARENA_ALIGN) * V.ARENA_ALIGN)
+        V.place_states(bufs, off)
         return V.VMProgram(
             arena_bytes=off, buffers=bufs,
             inputs=[t.buf for t in self.inputs],
@@ -640,3 +933,9 @@ class Graph:
 
 
 ARENA_SLOT = 64
+
+
+def rotary_grad_workers(T: int, H: int) -> int:
+    """Tiles of a rotary gradient, each with a partial sum of dweight of its own: one per
+    16 (row, head) pairs up to 256, a CU's worth each."""
+    return max(1, min(256, T * H // 16))

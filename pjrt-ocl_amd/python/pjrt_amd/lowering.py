@@ -914,7 +914,7 @@ def donation_aliases(prog: V.VMProgram, main: M.Func, cfg=None) -> list:
         reads = [phase[k] for k, ins in enumerate(prog.instrs)
                  if ins.op != V.OP_NOP and k in phase and grp[bi] in {grp[b] for b in passes.reads_of(ins, prog)}]
         writes = [phase[k] for k, ins in enumerate(prog.instrs)
-                  if ins.op != V.OP_NOP and k in phase and grp[bo] in {grp[b] for b in passes.writes_of(ins)}]
+                  if ins.op != V.OP_NOP and k in phase and grp[bo] in {grp[b] for b in passes.writes_of(ins, prog)}]
         if writes and (not reads or max(reads) < min(writes)):
             out.append((i, o))
     return out

@@ -79,12 +79,11 @@ def reads_of(ins: V.Instr, prog: V.VMProgram) -> set:
     return _instr_reads(ins, prog)
 
 
-def writes_of(ins: V.Instr) -> set:
+def writes_of(ins: V.Instr, prog: V.VMProgram) -> set:
     if ins.op in (V.OP_NOP, V.OP_FOR, V.OP_WHILE, V.OP_IF):
         return set()
-    if ins.op == V.OP_ARGMAX_SEG:
-        return {ins.dst, ins.b}
-    return {ins.dst}
+    from .scheduler import _instr_writes
+    return _instr_writes(ins, prog)
 
 
 def scopes(prog: V.VMProgram) -> list:
@@ -115,7 +114,7 @@ class _Index:
         for i, ins in enumerate(prog.instrs):
             if ins.op == V.OP_NOP:
                 continue
-            for b in writes_of(ins):
+            for b in writes_of(ins, prog):
                 self.writers.setdefault(b, []).append(i)
             for b in reads_of(ins, prog):
                 self.readers.setdefault(b, []).append(i)
@@ -251,7 +250,7 @@ def dce(prog: V.VMProgram) -> None:
         for i, ins in enumerate(prog.instrs):
             if ins.op == V.OP_NOP:
                 continue
-            if not live[i] and writes_of(ins) & live_buf:
+            if not live[i] and writes_of(ins, prog) & live_buf:
                 live[i] = True
                 changed = True
             if live[i]:
@@ -1688,7 +1687,7 @@ def reuse_arena(prog: V.VMProgram, cfg=None) -> None:
     for i, ins in enumerate(prog.instrs):
         if ins.op == V.OP_NOP or i not in phase:
             continue
-        for b in reads_of(ins, prog) | writes_of(ins):
+        for b in reads_of(ins, prog) | writes_of(ins, prog):
             touch(b, phase[i], order[i])
     end, end2 = n_ph, prog.main_len
     for b in set(prog.inputs):
@@ -1711,6 +1710,8 @@ def reuse_arena(prog: V.VMProgram, cfg=None) -> None:
         members.setdefault(group[b], []).append(b)
     units = []
     for root, mem in members.items():
+        if bufs[root].state:                # caller-owned memory, no arena bytes
+            continue
         base = min(bufs[m].arena_byte_offset for m in mem)
         top = max(bufs[m].arena_byte_offset + bufs[m].size_bytes for m in mem)
         l = min(lo[m] for m in mem)
@@ -1745,9 +1746,12 @@ def reuse_arena(prog: V.VMProgram, cfg=None) -> None:
                 new_off[m] = 0
                 bufs[m].size_bytes = 0
     for b in range(nb):
+        if bufs[b].state:
+            continue
         bufs[b].arena_byte_offset = new_off[b]
         arena_end = max(arena_end, new_off[b] + bufs[b].size_bytes)
     prog.arena_bytes = max(arena_end, V.ARENA_ALIGN)
+    V.place_states(bufs, prog.arena_bytes)
     if hasattr(prog, "_overlap_groups"):
         try:
             del prog._overlap_groups

@@ -312,6 +312,7 @@ class Runtime:
                                    err, _ERRLEN), err)
         lp = LoadedProgram(self, p)
         lp._blob = blob
+        lp.states = V.state_inputs(blob)
         self._programs.add(lp)
         return lp
 
@@ -439,6 +440,7 @@ class LoadedProgram:
         ni, no, nl = ctypes.c_uint32(), ctypes.c_uint32(), ctypes.c_uint32()
         lib.vmrt_program_counts(self._h, ctypes.byref(ni), ctypes.byref(no), ctypes.byref(nl))
         self.n_lanes = nl.value
+        self.states = ()                # indices of the inputs that a run writes in place
         self.inputs = [self._io(0, i) for i in range(ni.value)]
         self.outputs = [self._io(1, i) for i in range(no.value)]
 
@@ -526,11 +528,16 @@ class LoadedProgram:
                 "tasks": [(i, v[4 + 4 * i] / 100.0, v[5 + 4 * i] / 100.0, int(v[6 + 4 * i])) for i in range(n_tasks)]}
 
     def __call__(self, *args):
-        """Host convenience: numpy arrays in, numpy arrays out."""
+        """Host convenience: numpy arrays in, numpy arrays out.  The arrays of state
+        inputs (contiguous, of the buffer's own dtype) are updated in place."""
         self._live()
         if len(args) != len(self.inputs):
             raise VmrtError(INVALID_ARGUMENT, f"expected {len(self.inputs)} inputs, got {len(args)}")
         dev_in = []
+        for i in self.states:
+            a, spec = args[i], self.inputs[i]
+            if not (isinstance(a, np.ndarray) and a.flags.c_contiguous and a.flags.writeable and a.dtype == spec.np_dtype):
+                raise VmrtError(INVALID_ARGUMENT, f"state input {i} takes a writeable contiguous {spec.np_dtype} array")
         for a, spec in zip(args, self.inputs):
             a = np.ascontiguousarray(a)
             if spec.dtype == V.DT_BF16 and a.dtype != np.uint16:
@@ -544,6 +551,8 @@ class LoadedProgram:
             dev_in.append(self.rt.to_device(a))
         outs = self.execute(dev_in)
         res = [o.to_host(spec.np_dtype, spec.shape) for o, spec in zip(outs, self.outputs)]
+        for i in self.states:
+            args[i].reshape(-1)[:] = dev_in[i].to_host(self.inputs[i].np_dtype)
         for b in dev_in + outs:
             b.free()
         return res

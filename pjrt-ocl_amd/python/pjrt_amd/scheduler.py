@@ -194,6 +194,14 @@ def n_tiles(task: V.Task, cfg: DeviceConfig) -> int:
         return max(1, task.p3) * -(-task.p1 // task.p4)
     if top == V.TOP_DECODE_ATTN:
         return max(1, (task.p4 & 0xFFFF) * max(1, task.p4 >> 16))
+    if top == V.TOP_ROTARY:
+        return max(1, -(-task.p4 * task.p3 // 4))
+    if top == V.TOP_ROTARY_GRAD:
+        return max(1, task.p3)
+    if top in (V.TOP_CACHE_APPEND, V.TOP_CACHE_READ):
+        return max(1, -(-(task.p7 >> 8) // (task.p7 & 0xFF)))
+    if top == V.TOP_PAGED_ATTN:
+        return max(1, task.p7)
     raise ScheduleError(f"n_tiles: unknown tile_op {top}")
 
 
@@ -286,6 +294,21 @@ def red_splits(n_out: int, red: int, dt: int, cfg: DeviceConfig) -> int:
     while s < 64 and blocks * s * 2 <= cfg.nlanes and red >= 256 * s:
         s *= 2
     return s
+
+
+def rotary_splits(T: int, H: int, cfg: DeviceConfig) -> int:
+    """Head splits of a TOP_ROTARY row (p3): a wave takes a row's heads of one split, so
+    few rows are cut until every wave of the lanes has work or a split is four heads."""
+    z = 1
+    while T * z * 2 <= 4 * cfg.nlanes and H >= 8 * z:
+        z *= 2
+    return z
+
+
+def cache_rows_per_tile(T: int, cfg: DeviceConfig) -> int:
+    """Rows of a TOP_CACHE_APPEND / READ tile: the share of a lane, at most 64 (a wave
+    looks 64 rows' places up at once)."""
+    return max(1, min(64, -(-T // cfg.nlanes)))
 
 
 def argmax_splits(n_out: int, seg: int, cfg: DeviceConfig) -> int:
@@ -479,6 +502,19 @@ def instr_to_task(ins: V.Instr, prog: V.VMProgram, cfg: DeviceConfig) -> V.Task:
         S = decode_splits(ins.n, ins.imm, cfg)
         t = V.Task(V.TOP_DECODE_ATTN, ins.dst, ins.a, ins.b, ins.imm2, kb, vb,
                    posb, ins.n | (S << 16), hd, ins.imm, sbits)
+    elif op == V.OP_ROTARY:
+        freq = prog.aux[ins.aux + 13]
+        t = V.Task(V.TOP_ROTARY, ins.dst, ins.a, ins.b, ins.imm2, freq, ins.aux,
+                   rotary_splits(ins.n, ins.imm, cfg), ins.n)
+    elif op == V.OP_ROTARY_GRAD:
+        freq, weight, part, workers = prog.aux[ins.aux + 13:ins.aux + 17]
+        t = V.Task(V.TOP_ROTARY_GRAD, ins.dst, ins.a, ins.b, ins.imm2, freq, ins.aux, workers, weight, part)
+    elif op in V.CACHE_OPS:
+        bufs6 = prog.aux[ins.aux + 17:ins.aux + 23]
+        top, p7 = {V.OP_CACHE_APPEND: (V.TOP_CACHE_APPEND, ins.n << 8 | cache_rows_per_tile(ins.n, cfg)),
+                   V.OP_CACHE_READ: (V.TOP_CACHE_READ, ins.n << 8 | cache_rows_per_tile(ins.n, cfg)),
+                   V.OP_PAGED_ATTN: (V.TOP_PAGED_ATTN, cfg.nlanes)}[op]
+        t = V.Task(top, ins.dst, ins.a, ins.b, *bufs6, ins.aux, p7)
     elif op == V.OP_DOT:
         M, N, K, G = ins.n, ins.imm >> 16, ins.imm & 0xFFFF, max(1, ins.imm2)
         aview, bview, epi, epi_res = ins.aview, ins.bview, ins.epi, ins.epi_res
@@ -736,6 +772,17 @@ def _instr_reads(ins: V.Instr, prog: V.VMProgram) -> set:
         r = {ins.a, ins.b, ins.imm2}
     elif op == V.OP_DECODE_ATTN:
         r = {ins.a, ins.b, ins.imm2} | set(prog.aux[ins.aux + 1:ins.aux + 4])
+    elif op == V.OP_ROTARY:
+        r = {ins.a, ins.b, ins.imm2, prog.aux[ins.aux + 13]}
+    elif op == V.OP_ROTARY_GRAD:
+        r = {ins.a, ins.b, ins.imm2, *prog.aux[ins.aux + 13:ins.aux + 15]}
+    elif op in V.CACHE_OPS:
+        # the pages and scales that append writes keep the rest of what they hold
+        r = {ins.a, ins.b, *prog.aux[ins.aux + 17:ins.aux + 23]}
+        if op == V.OP_CACHE_READ:
+            r -= {prog.aux[ins.aux + 17]}
+        else:
+            r |= {ins.dst} if op == V.OP_CACHE_APPEND else set()
     elif op == V.OP_MAP_REGION:
         r = set(ins.region_inputs or _region_inputs_from_aux(ins, prog))
     elif op in (V.OP_DYNAMIC_SLICE, V.OP_DYNAMIC_UPDATE_SLICE, V.OP_GATHER_INDEX):
@@ -761,6 +808,13 @@ def _instr_writes(ins: V.Instr, prog: V.VMProgram) -> set:
         return set()
     if ins.op == V.OP_ARGMAX_SEG:
         return {ins.dst, ins.b}
+    if ins.op == V.OP_ROTARY_GRAD:
+        return {ins.dst, prog.aux[ins.aux + 15]}
+    if ins.op == V.OP_CACHE_APPEND:
+        w = {ins.dst, prog.aux[ins.aux + 17]}
+        return w | set(prog.aux[ins.aux + 18:ins.aux + 20]) if prog.aux[ins.aux + 8] == V.DT_I8 else w
+    if ins.op == V.OP_CACHE_READ:
+        return {ins.dst, prog.aux[ins.aux + 17]}
     return {ins.dst}
 
 
@@ -768,6 +822,24 @@ def _instr_writes(ins: V.Instr, prog: V.VMProgram) -> set:
 
 _HBM_GBS = 5000.0          # effective GB/s assumed before calibration
 _MFMA_TFLOPS = 1200.0
+
+
+def _extension_work(task: V.Task, prog: V.VMProgram):
+    """(HBM bytes, flops) of a rotary or paged cache task, None for others.  How long
+    the sequences are is known on the device only: attention is taken to read half of
+    what the table can hold, once per sequence."""
+    top, aux = task.tile_op, prog.aux
+    if top in (V.TOP_ROTARY, V.TOP_ROTARY_GRAD):
+        T, H, hd = aux[task.p2:task.p2 + 3]
+        return T * H * hd * V.DT_SIZE[task.dtype] * (2 if top == V.TOP_ROTARY else 3), 0.0
+    if top in (V.TOP_CACHE_APPEND, V.TOP_CACHE_READ):
+        T, _, Hkv, hd = aux[task.p6:task.p6 + 4]
+        return 2 * T * Hkv * hd * (V.DT_SIZE[task.dtype] + V.DT_SIZE[task.adtype]), 0.0
+    if top == V.TOP_PAGED_ATTN:
+        T, Hq, Hkv, hd, P, _, B, MP, cdt = aux[task.p6:task.p6 + 9]
+        keys = max(1, MP * P // 2)
+        return 2 * B * keys * Hkv * hd * V.DT_SIZE[cdt], 4.0 * T * Hq * hd * keys
+    return None
 
 
 def task_cost(task: V.Task, cfg: DeviceConfig, prog: V.VMProgram) -> float:
@@ -797,6 +869,9 @@ def task_cost(task: V.Task, cfg: DeviceConfig, prog: V.VMProgram) -> float:
         # each tile streams its share of a head's two cache slices (~15 GB/s per CU)
         H, S = task.p4 & 0xFFFF, max(1, task.p4 >> 16)
         return H * S * (2.0 * (task.p5 & 0xFFFF) * task.p6 * asz / S / 15e3 + 3.0)
+    ext = _extension_work(task, prog)
+    if ext:
+        return max(ext[1] / (_MFMA_TFLOPS * 1e6), ext[0] / (_HBM_GBS * 1e3)) + 2.0
     if top in (V.TOP_RED_SEG, V.TOP_SOFTMAX_SEG, V.TOP_LAYERNORM_SEG,
                V.TOP_ARGMAX_SEG):
         n = task.p0 * task.p1
@@ -833,6 +908,9 @@ def task_work(task: V.Task, prog: V.VMProgram) -> tuple:
         return 2 * H * C * hd * asz, 4.0 * H * T * C * hd
     if top == V.TOP_DECODE_ATTN:
         return 2 * (task.p4 & 0xFFFF) * (task.p5 & 0xFFFF) * task.p6 * asz, 0.0
+    ext = _extension_work(task, prog)
+    if ext:
+        return ext
     if top in (V.TOP_RED_SEG, V.TOP_SOFTMAX_SEG, V.TOP_LAYERNORM_SEG, V.TOP_ARGMAX_SEG):
         return task.p0 * task.p1 * (asz + (dsz if top != V.TOP_RED_SEG else 0)), 0.0
     n = max(task.p0, task.p1) if top != V.TOP_EW else task.p1
@@ -1140,7 +1218,7 @@ class _Scheduler:
                           # neighbouring strips share weight lines (a 16-column
                           # bf16 strip is a quarter of a 128-byte line): on one
                           # XCD they share its L2 (C5: 1014 -> 1036 tokens/s)
-                          t.tile_op in (V.TOP_FLASH_ATTN, V.TOP_GEMV)))
+                          t.tile_op in (V.TOP_FLASH_ATTN, V.TOP_GEMV, V.TOP_PAGED_ATTN)))
         for comp in self.chains(maps):
             tids = [self.task_id(i) for i in comp]
             t0 = self.tasks[tids[0]]

@@ -57,6 +57,25 @@ which does not use them is byte-for-byte a reference program):
   decoder's form that stores k, v at pos before attending over keys <= pos:
   pos is clamped to [0, C - 1] and a negative pos gives a NaN output.
 
+* element type ``i8`` (8): pages of a paged cache only.
+* a buffer entry's pad word 1 (``BUF_STATE``): an input of the program that its
+  tasks write in place.  The buffer is caller-owned memory bound as a port; it
+  takes no arena bytes and its offset lies past them, so it may be larger than the
+  arena's 2 GiB.
+* tensor opcodes ``OP_ROTARY`` (69) and ``OP_ROTARY_GRAD`` (70) / tile ops 22, 23:
+  rotary positions of the heads of [T, H, hd] rows, with an optional RMS norm of
+  each head before.  Task: a x (gradient: a dy, b x), b weight (gradient: p4), p0
+  positions, p1 frequencies (u32 pairs, 64-bit fixed-point turns per position), p2
+  descriptor (``RD_*`` words of vm_abi.h), p3 head splits Z; tile = four (row, split)
+  pairs.  Gradient: p3 workers, p5 partial sums of dweight [p3, hd]; tile = worker.
+* ``OP_CACHE_APPEND`` (71), ``OP_CACHE_READ`` (72), ``OP_PAGED_ATTN`` (73) / tile ops
+  24, 25, 26: new rows into the pages of a cache, the rows of a batch back out of
+  it, and attention over it.  Instr: aux -> the descriptor (``PD_*`` words), then
+  the buffers [V pages (read: v out), k scales, v scales, cu, lens, table].  Task:
+  p0-p5 those buffers, p6 descriptor, p7 rows per tile (append, read) or workers
+  (attention); a, b = k, v new rows and dst = K pages (append), a, b = K, V pages and
+  dst, p0 = k, v out (read), a, b = q, K pages (attention).
+
 Task scratch: the loader gives each task that needs it (a split decode
 attention or argmax) its own zeroed region of device memory; the last split of
 a head / row resets its arrival counter, so the region is zero again for the
@@ -79,18 +98,20 @@ SECTION_ALIGN = 8
 
 # ---- dtypes (lowering.py:59-81) ---------------------------------------------
 DT_F32, DT_I32, DT_U32, DT_BOOL, DT_I64, DT_F64, DT_F16, DT_BF16 = range(8)
-DT_MAX = DT_BF16
+DT_I8 = 8                    # extension: pages of a paged cache only
+DT_MAX = DT_I8
 DT_NAMES = {DT_F32: "f32", DT_I32: "i32", DT_U32: "u32", DT_BOOL: "bool",
-            DT_I64: "i64", DT_F64: "f64", DT_F16: "f16", DT_BF16: "bf16"}
+            DT_I64: "i64", DT_F64: "f64", DT_F16: "f16", DT_BF16: "bf16", DT_I8: "i8"}
 DT_BY_NAME = {v: k for k, v in DT_NAMES.items()}
 DT_SIZE = {DT_F32: 4, DT_I32: 4, DT_U32: 4, DT_BOOL: 1, DT_I64: 8, DT_F64: 8,
-           DT_F16: 2, DT_BF16: 2}
+           DT_F16: 2, DT_BF16: 2, DT_I8: 1}
 # numpy storage dtype for each element type; bf16 is carried as its raw 16-bit
 # pattern (uint16) because numpy has no bfloat16 (see f32_to_bf16/bf16_to_f32).
 DT_NUMPY = {DT_F32: np.dtype("<f4"), DT_I32: np.dtype("<i4"),
             DT_U32: np.dtype("<u4"), DT_BOOL: np.dtype("u1"),
             DT_I64: np.dtype("<i8"), DT_F64: np.dtype("<f8"),
-            DT_F16: np.dtype("<f2"), DT_BF16: np.dtype("<u2")}
+            DT_F16: np.dtype("<f2"), DT_BF16: np.dtype("<u2"),
+            DT_I8: np.dtype("i1")}
 FLOAT_DTYPES = frozenset({DT_F32, DT_F64, DT_F16, DT_BF16})
 
 
@@ -159,7 +180,9 @@ OP_SCATTER_INDEX = 65
 OP_LAYERNORM_AFFINE = 66
 OP_ARGMAX_SEG = 67
 OP_DECODE_ATTN = 68
-OP_MAX = OP_DECODE_ATTN
+OP_ROTARY, OP_ROTARY_GRAD, OP_CACHE_APPEND, OP_CACHE_READ, OP_PAGED_ATTN = range(69, 74)
+OP_MAX = OP_PAGED_ATTN
+CACHE_OPS = frozenset({OP_CACHE_APPEND, OP_CACHE_READ, OP_PAGED_ATTN})
 
 REGION_OPS = frozenset({OP_WHILE, OP_IF, OP_FOR})
 
@@ -172,7 +195,8 @@ TOP_EW, TOP_MMA, TOP_GATHER, TOP_RED_PART, TOP_RED_COMB, TOP_IOTA_DIM, \
 TOP_ARGMAX_SEG = 19          # extension
 TOP_GEMV = 20                # extension
 TOP_DECODE_ATTN = 21         # extension
-TOP_MAX = TOP_DECODE_ATTN
+TOP_ROTARY, TOP_ROTARY_GRAD, TOP_CACHE_APPEND, TOP_CACHE_READ, TOP_PAGED_ATTN = range(22, 27)   # extensions
+TOP_MAX = TOP_PAGED_ATTN
 
 # ---- EW subops (vm_common.cl:118-146) ------------------------------------------
 SUB_ADD, SUB_MUL, SUB_SUB, SUB_DIV, SUB_MAX, SUB_MIN, SUB_POW, SUB_COPY, \
@@ -203,6 +227,14 @@ RED_SUM, RED_MAX, RED_MIN, RED_PROD, RED_AND, RED_OR, RED_XOR = range(7)
 LN_AFFINE = 1     # y = y * gamma[col] + beta[col]; gamma = task.b, beta = task.p4
 LN_GELU = 2       # y = gelu_tanh(y)
 LN_TWO_PASS = 4   # variance as mean((x - mu)^2) instead of E[x^2] - mu^2
+
+# ROTARY descriptor flags (extension)
+ROT_INTERLEAVED, ROT_NORM, ROT_INVERSE = 1, 2, 4
+# paged attention: query heads per kv head, rows of one block of queries at most
+PAGED_MAX_GROUP = 128
+PAGED_MAX_ROWS = 256
+# buffer entry pad word (extension): caller-owned memory, written in place
+BUF_STATE = 1
 
 # MMA task p3: batch count in bits 0..23, tile-edge code in bits 24..27
 MMA_TILE_CODES = {0: 0, 64: 1, 128: 2, 256: 3}
@@ -239,6 +271,9 @@ class Buffer:
     arena_byte_offset: int
     size_bytes: int
     dtype: int = DT_F32
+    # an input that tasks write in place: caller-owned memory bound as a port,
+    # its offset past the arena (so it overlaps no other buffer)
+    state: bool = False
 
     @property
     def n_elems(self) -> int:
@@ -303,6 +338,16 @@ class Entry:
     pad: int = 0
 
 
+def place_states(buffers: list, arena_bytes: int) -> None:
+    """Offsets of the state buffers: one after another past the arena, where they
+    overlap nothing (the loader binds them as ports and reads no offset of theirs)."""
+    off = -(-arena_bytes // ARENA_ALIGN) * ARENA_ALIGN
+    for b in buffers:
+        if b.state:
+            b.arena_byte_offset = off
+            off += max(ARENA_ALIGN, -(-b.size_bytes // ARENA_ALIGN) * ARENA_ALIGN)
+
+
 def barrier_entry() -> Entry:
     return Entry(ENT_BARRIER)
 
@@ -364,7 +409,7 @@ def serialize(prog: VMProgram, schedule: Schedule | None = None) -> bytes:
     for b in prog.buffers:
         if b.arena_byte_offset % ARENA_ALIGN:
             raise FormatError(f"buffer offset {b.arena_byte_offset} not aligned")
-        out += BUFENT.pack(b.arena_byte_offset, b.size_bytes, b.dtype, 0)
+        out += BUFENT.pack(b.arena_byte_offset, b.size_bytes, b.dtype, BUF_STATE if b.state else 0)
     for ids in (prog.inputs, prog.outputs):
         for i in ids:
             out += struct.pack("<I", i)
@@ -438,13 +483,13 @@ def parse(data: bytes) -> VMProgram:
     for i in range(n_buffers):
         off, size, dt, pad = BUFENT.unpack_from(data, pos)
         pos += BUFENT.size
-        if off % ARENA_ALIGN or off + size > arena_bytes:
+        if pad not in (0, BUF_STATE):
+            raise FormatError(f"buffer {i} pad nonzero")
+        if off % ARENA_ALIGN or (off < arena_bytes if pad else off + size > arena_bytes):
             raise FormatError(f"buffer {i} outside arena / misaligned")
         if dt > DT_MAX:
             raise FormatError(f"buffer {i} unsupported dtype {dt}")
-        if pad:
-            raise FormatError(f"buffer {i} pad nonzero")
-        buffers.append(Buffer(off, size, dt))
+        buffers.append(Buffer(off, size, dt, bool(pad)))
 
     def ids(count: int, what: str) -> list:
         nonlocal pos
@@ -458,6 +503,9 @@ def parse(data: bytes) -> VMProgram:
 
     inputs = ids(n_inputs, "input")
     outputs = ids(n_outputs, "output")
+    for i, b in enumerate(buffers):
+        if b.state and (inputs.count(i) != 1 or i in outputs):
+            raise FormatError(f"state buffer {i} is not an input of its own")
 
     def shape() -> tuple:
         nonlocal pos
@@ -515,6 +563,14 @@ def parse(data: bytes) -> VMProgram:
     if pos != len(data):
         raise FormatError(f"trailing bytes: parsed {pos} of {len(data)}")
     return prog
+
+
+def state_inputs(data: bytes) -> tuple:
+    """Indices of a program's inputs that are state buffers."""
+    n_buffers, n_inputs = HEADER.unpack_from(data, 0)[2], HEADER.unpack_from(data, 0)[6]
+    pad = np.frombuffer(data, "<u4", 6 * n_buffers, HEADER.size).reshape(n_buffers, 6)[:, 5]
+    ids = np.frombuffer(data, "<u4", n_inputs, HEADER.size + BUFENT.size * n_buffers)
+    return tuple(int(i) for i in np.nonzero(pad[ids] == BUF_STATE)[0])
 
 
 def _parse_schedule(data: bytes, pos: int, n_buffers: int, n_aux: int):
