@@ -1408,7 +1408,7 @@ def _instr_task(prog: Prog, ins, ew_ts: int, mma_t: int):
         top, p = 23, [imm2, freq, aux, workers, weight, part, 0, 0]
     elif op in (71, 72, 73):
         top = 24 + op - 71
-        p = list(prog.aux[aux + 17:aux + 23]) + [aux, n << 8 | 64 if op < 73 else 1]
+        p = list(prog.aux[aux + 25:aux + 31]) + [aux, n << 8 | 64 if op < 73 else 1]
     elif op == 27:
         M, N, K, G = n, imm >> 16, imm & 0xFFFF, max(1, imm2)
         views = prog.aux[aux:aux + 4] if aux else [0, 0, 0, 0]

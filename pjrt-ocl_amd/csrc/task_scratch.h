@@ -51,7 +51,8 @@ inline uint64_t task_scratch_bytes(const Task& t, uint32_t mma_t) {
 inline uint64_t paged_scratch_bytes(const Task& t, const int32_t* aux) {
   const int32_t* d = aux + t.p[6];
   const uint64_t rows = std::min<uint64_t>(kPagedMaxRows, uint64_t(d[PD_T]) * (d[PD_HQ] / d[PD_HKV]));
-  return (2 * rows * (uint64_t(d[PD_HD]) + 2) + 1) * t.p[7] * 4;
+  const uint64_t slot = (rows * (uint64_t(d[PD_HD]) + 2) + 3) & ~uint64_t(3);
+  return (2 * slot + 1) * t.p[7] * 4;
 }
 
 }  // namespace vm

@@ -30,18 +30,21 @@ struct PagedDesc {
   uint32_t ars, ahs, aoff, brs, bhs, boff;
   float scale;
   uint32_t window;
+  DivU32 dp, dg;       // by P, by Hq / Hkv
 };
 VM_DEV PagedDesc paged_desc(Args A, const VM_K Task& t) {
   const VM_K int32_t* d = aux_of(A) + t.p[6];
   return PagedDesc{uint32_t(d[PD_T]), uint32_t(d[PD_HQ]), uint32_t(d[PD_HKV]), uint32_t(d[PD_HD]), uint32_t(d[PD_PAGE]),
                    uint32_t(d[PD_PAGES]), uint32_t(d[PD_SEQS]), uint32_t(d[PD_MAXP]), uint32_t(d[PD_CDT]),
                    uint32_t(d[PD_ARS]), uint32_t(d[PD_AHS]), uint32_t(d[PD_AOFF]), uint32_t(d[PD_BRS]),
-                   uint32_t(d[PD_BHS]), uint32_t(d[PD_BOFF]), __int_as_float(d[PD_SCALE]), uint32_t(d[PD_WINDOW])};
+                   uint32_t(d[PD_BHS]), uint32_t(d[PD_BOFF]), __int_as_float(d[PD_SCALE]), uint32_t(d[PD_WINDOW]),
+                   DivU32{uint32_t(d[PD_DIVP]), uint32_t(d[PD_DIVP + 1]), uint32_t(d[PD_DIVP + 2]), uint32_t(d[PD_DIVP + 3])},
+                   DivU32{uint32_t(d[PD_DIVG]), uint32_t(d[PD_DIVG + 1]), uint32_t(d[PD_DIVG + 2]), uint32_t(d[PD_DIVG + 3])}};
 }
 
 constexpr uint64_t kNoPlace = ~uint64_t(0);
 
-// Place of row r (each lane its own): page * P + slot, or kNoPlace.  Every lane of the
+// Place of row r (each lane its own): page and slot in the halves, or kNoPlace.  Every lane of the
 // wave calls it.
 VM_DEV uint64_t row_place(const PagedDesc& D, const VM_G int32_t* cu, const VM_G int32_t* lens,
                           const VM_G int32_t* table, uint32_t r) {
@@ -58,9 +61,10 @@ VM_DEV uint64_t row_place(const PagedDesc& D, const VM_G int32_t* cu, const VM_G
   const uint32_t cap = D.MP * D.P;
   if (len < c1 - c0 || uint32_t(len) > cap) return kNoPlace;
   const uint32_t p = uint32_t(len) - (uint32_t(c1) - r);
-  const int32_t page = table[uint64_t(s) * D.MP + p / D.P];
+  const uint32_t e = D.dp.quo(p);
+  const int32_t page = table[uint64_t(s) * D.MP + e];
   if (page < 0 || uint32_t(page) >= D.N) return kNoPlace;
-  return uint64_t(page) * D.P + p % D.P;
+  return (uint64_t(page) << 32) | (p - e * D.P);
 }
 
 // Eight signed bytes as f32 and back.
@@ -127,8 +131,7 @@ VM_TILE void cache_move(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
         ok[k] = u < total && p != kNoPlace;
         const uint64_t pp = p == kNoPlace ? 0 : p;
         // element of the pages [N, heads, P, hd]; scales [N, heads, P] share the row index
-        const uint64_t page = pp / D.P;
-        at[k] = (page * D.Hkv + h[k]) * D.P + (pp - page * D.P);
+        at[k] = (uint64_t(uint32_t(pp >> 32)) * D.Hkv + h[k]) * D.P + uint32_t(pp);
         row[k] = READ ? (uint64_t(r0 + r) * D.Hkv + h[k]) * D.hd
                       : kv[k] ? uint64_t(r0 + r) * D.brs + uint64_t(h[k]) * D.bhs + D.boff
                               : uint64_t(r0 + r) * D.ars + uint64_t(h[k]) * D.ahs + D.aoff;

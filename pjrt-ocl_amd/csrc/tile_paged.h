@@ -13,26 +13,28 @@
 // workers (p7, one per lane) that divide the step among themselves.  A sequence's new
 // tokens are cut into blocks of TB tokens; an item is one block of one kv head, its rows
 // all (token, query head of the group) pairs, its keys [kstart, kend) from the first
-// position its first token sees to its last token's own.  An item costs kItemCost +
-// its keys; with C the sum over all items, in the order sequence, head, block, worker w
-// takes cost [w C / W, (w + 1) C / W).  An item that lies across workers is cut at
-// multiples of kKeyAlign keys: each piece leaves its rows' (max, sum, O) in the task's
+// position its first token sees to its last token's own.  An item costs kItemCost plus
+// its keys times the block's weight (what a key costs a block of its rows); with C the
+// sum over all items, in the order sequence, head, block, worker w takes cost
+// [w C / W, (w + 1) C / W).  An item that lies across workers is cut, unless that is near
+// its start or end: each piece leaves its rows' (max, sum, O) in the task's
 // scratch, and the piece that arrives last at the item's counter joins them in key
 // order.  So one long sequence and many short ones keep every CU as busy, the result
 // depends on the lengths alone, and nothing waits.
 //
-// Scratch: 2 W slots of kPagedMaxRows' (or T g) rows x (hd + 2) floats: worker w's first
-// item in slot 2 w, its last in 2 w + 1; then W arrival counters, by the worker that
-// holds the item's first cost.
+// Scratch: 2 W slots of kPagedMaxRows' (or T g) rows x (hd + 2) floats: worker w's piece of
+// an item that begins before it in slot 2 w, of one that ends after it in 2 w + 1; then W
+// arrival counters, by the worker of the item's first piece.
 #pragma once
 #include "tile_attn.h"
 #include "tile_cache.h"
 
 namespace vm {
 
-constexpr uint32_t kItemCost = 96;         // an item's fixed cost in keys
-constexpr uint32_t kKeyAlign = 128;        // pieces of an item are multiples of this many keys
-constexpr uint32_t kMinShare = 256;        // cost of a worker at least (> kItemCost + kKeyAlign: see pieces())
+// Costs are in units of about 12.5 ns of one CU: what a key of 128 channels costs a block of
+// 64 rows on the matrix cores, half of what streaming it from HBM costs (all CUs at once).
+constexpr uint32_t kItemCost = 192;        // an item's fixed cost
+constexpr uint32_t kMinShare = 512;        // cost of a worker at least
 
 struct PagedSeq {                          // a sequence with new rows and a place for them
   uint32_t r0, n, len, p0;                 // first row, rows, length, first row's position
@@ -51,26 +53,31 @@ VM_DEV bool paged_seq(const PagedDesc& D, int32_t c0, int32_t c1, int32_t len, P
 
 // Blocks of a sequence: key ranges and the cost of the first b blocks of a head.
 struct PagedBlocks {
-  uint32_t tb, nb, n, p0, len, window;
-  VM_DEV uint32_t kend(uint32_t b) const { return p0 + min(n, (b + 1) * tb); }
-  VM_DEV uint32_t kstart(uint32_t b) const {
-    if (!window) return 0;
-    const int64_t k = int64_t(p0) + int64_t(b) * tb + 1 - window;
-    return k > 0 ? uint32_t(k) : 0u;
-  }
-  // sum over i < b of kItemCost + kend(i) - kstart(i)
-  VM_DEV uint64_t before(uint32_t b) const {
-    uint64_t c = uint64_t(b) * (kItemCost + p0) + uint64_t(tb) * (uint64_t(b) * (b + 1) / 2);
-    if (b == nb) c -= uint64_t(nb) * tb - n;                       // the last block's end is the length
+  uint32_t tb, nb, n, p0, weight, align;   // cut at multiples of `align` keys; weight a power of two
+  int32_t a;                     // kstart(b) = max(0, a + b tb)
+  uint32_t i0;                   // the first b with a + b tb > 0
+  VM_DEV void set(const PagedSeq& q, uint32_t window) {
+    nb = q.n <= tb ? 1u : (q.n + tb - 1) / tb;
+    n = q.n;
+    p0 = q.p0;
+    a = INT32_MIN;
+    i0 = 0xFFFFFFFFu;
     if (window) {
-      const int64_t a = int64_t(p0) + 1 - window;                  // kstart(i) = max(0, a + i tb)
-      const uint64_t i0 = a > 0 ? 0 : uint64_t(-a) / tb + 1;       // the first i with a + i tb > 0
-      if (b > i0) {
-        const uint64_t cnt = b - i0;
-        c -= cnt * uint64_t(a + int64_t(i0 * tb)) + uint64_t(tb) * (cnt * (cnt - 1) / 2);
-      }
+      a = int32_t(p0) + 1 - int32_t(window);
+      i0 = a > 0 ? 0u : uint32_t(-a) / tb + 1;
     }
-    return c;
+  }
+  VM_DEV uint32_t kend(uint32_t b) const { return p0 + min(n, (b + 1) * tb); }
+  VM_DEV uint32_t kstart(uint32_t b) const { return b < i0 ? 0u : uint32_t(a + int32_t(b * tb)); }
+  // sum over i < b of kItemCost + weight (kend(i) - kstart(i))
+  VM_DEV uint64_t before(uint32_t b) const {
+    uint64_t c = uint64_t(b) * p0 + uint64_t(tb) * (uint64_t(b) * (b + 1) / 2);
+    if (b == nb) c -= nb * tb - n;                               // the last block's end is the length
+    if (b > i0) {
+      const uint64_t cnt = b - i0;
+      c -= cnt * uint32_t(a + int32_t(i0 * tb)) + uint64_t(tb) * (cnt * (cnt - 1) / 2);
+    }
+    return c * weight + uint64_t(b) * kItemCost;
   }
 };
 
@@ -79,20 +86,23 @@ struct PagedJob {
   uint32_t seq, head, row0, tokens, pos0;  // rows row0 .. + tokens - 1 of the step, at positions pos0 ..
   uint32_t k0, k1;                         // its keys
   float* part;                             // its partial slot (null: the whole item, written to the output)
+  // a job passed to a function arrives in vector registers
+  VM_DEV void uniform() {
+    seq = uni(seq);
+    head = uni(head);
+    row0 = uni(row0);
+    tokens = uni(tokens);
+    pos0 = uni(pos0);
+    k0 = uni(k0);
+    k1 = uni(k1);
+    part = uni_ptr(part);
+  }
 };
-
-VM_DEV void agent_store(float* p, float v) {
-  __hip_atomic_store(reinterpret_cast<uint32_t*>(p), __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-VM_DEV float agent_load(const float* p) {
-  return __uint_as_float(
-      __hip_atomic_load(reinterpret_cast<const uint32_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-}
 
 // Partial slot of R rows: O [R][hd], then maxima [R] (base 2, scaled) and sums [R].
 VM_DEV uint64_t paged_slot_floats(const PagedDesc& D) {
   const uint64_t rows = uint64_t(D.T) * (D.Hq / D.Hkv);
-  return (rows < kPagedMaxRows ? rows : kPagedMaxRows) * (D.hd + 2);
+  return ((rows < kPagedMaxRows ? rows : kPagedMaxRows) * (D.hd + 2) + 3) & ~uint64_t(3);   // whole 16 bytes
 }
 
 // Zeros in the rows that no valid sequence has, a share per worker.
@@ -117,52 +127,112 @@ VM_DEV void paged_zero_rows(Args A, const VM_K Task& t, const PagedDesc& D, uint
 }
 
 // Join the pieces of an item: R rows, np partials, piece i in slot(i).  Every thread of
-// the block calls it, after the last arrival.
+// the block calls it, after the last arrival.  Each row's weights first (a thread a row,
+// into LDS), then a thread takes four channels of a row; the pieces' loads are issued
+// eight at a time (one after another they cost a memory round trip each: a 256-row item
+// of three pieces took 60 us to join, with them together 8).
 template <class Slot, class Row>
 VM_DEV void paged_join(Args A, const VM_K Task& t, const PagedDesc& D, uint32_t R, uint32_t np, Slot slot, Row row_at) {
-  const uint32_t dt = (t.tile_op >> 8) & 0xFF, hd = D.hd;
+  const uint32_t dt = (t.tile_op >> 8) & 0xFF, hd = D.hd, per = hd / 4, tid = threadIdx.x;
   gbyte* out = resolve(A, t.dst);
-  // a thread owns channels d, d + cols, ... of rows r, r + rpp, ...
-  const uint32_t cols = min(256u, pow2_at_least(hd)), rpp = kBlock / cols;
-  const uint32_t d0 = threadIdx.x % cols;
-  for (uint32_t r = threadIdx.x / cols; r < R; r += rpp) {
-    float M = -INFINITY;
-    for (uint32_t i = 0; i < np; ++i) M = fmaxf(M, agent_load(slot(i) + uint64_t(R) * hd + r));
-    float L = 0.0f, O = 0.0f;
-    for (uint32_t i = 0; i < np; ++i) {
-      const float* p = slot(i);
-      const float m = agent_load(p + uint64_t(R) * hd + r), l = agent_load(p + uint64_t(R) * (hd + 1) + r);
-      const float o = d0 < hd ? agent_load(p + uint64_t(r) * hd + d0) : 0.0f;
-      const float a = m == -INFINITY ? 0.0f : exp2f(m - M);
-      L = fmaf(l, a, L);
-      O = fmaf(o, a, O);
+  float* wt = lds_ptr<float>();                          // [np][rows of the round]
+  const uint32_t rc = min(R, 32768u / np);               // np <= 4096 workers
+  constexpr uint32_t U = 8;
+  for (uint32_t r0 = 0; r0 < R; r0 += rc) {
+    const uint32_t rows = min(rc, R - r0);
+    __syncthreads();
+    for (uint32_t r = tid; r < rows; r += kBlock) {
+      const uint64_t at = uint64_t(R) * hd + r0 + r;
+      float M = -INFINITY, L = 0.0f;
+      for (uint32_t i0 = 0; i0 < np; i0 += U) {
+        float m[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) m[u] = slot(min(i0 + u, np - 1))[at];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+          M = fmaxf(M, m[u]);
+          if (i0 + u < np) wt[(i0 + u) * rows + r] = m[u];
+        }
+      }
+      for (uint32_t i0 = 0; i0 < np; i0 += U) {
+        float l[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) l[u] = slot(min(i0 + u, np - 1))[at + R];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+          if (i0 + u < np) {
+            float* w = wt + (i0 + u) * rows + r;
+            const float a = *w == -INFINITY ? 0.0f : exp2f(*w - M);
+            L = fmaf(l[u], a, L);
+            *w = a;
+          }
+      }
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;     // a row that saw nothing is 0
+      for (uint32_t i = 0; i < np; ++i) wt[i * rows + r] *= inv;
     }
-    if (d0 < hd) store_f(out, dt, row_at(r) + d0, L == 0.0f ? 0.0f : O / L);
+    __syncthreads();
+    for (uint32_t x = tid; x < rows * per; x += kBlock) {
+      const uint32_t r = x / per, d = x % per * 4;
+      v4f O = v4f_make(0, 0, 0, 0);
+      for (uint32_t i0 = 0; i0 < np; i0 += U) {
+        v4f o[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) o[u] = *(const v4f*)(slot(min(i0 + u, np - 1)) + uint64_t(r0 + r) * hd + d);
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+          const float a = i0 + u < np ? wt[(i0 + u) * rows + r] : 0.0f;
+          if (i0 + u < np)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[e] = fmaf(o[u][e], a, O[e]);
+        }
+      }
+      const uint64_t at = row_at(r0 + r) + d;
+      const float f[4] = {O[0], O[1], O[2], O[3]};
+      if (dt == DT_F32) {
+        Run<DT_F32, 4> q;
+        q.put(f);
+        q.store(out, at);
+      } else if (dt == DT_BF16) {
+        Run<DT_BF16, 4> q;
+        q.put(f);
+        q.store(out, at);
+      } else {
+        Run<DT_F16, 4> q;
+        q.put(f);
+        q.store(out, at);
+      }
+    }
   }
 }
 
-// Worker w's share: its items' pieces one after another.  tokens_per_block(n) -> TB;
-// body(job) computes a piece (every thread of the block).
-template <class Tokens, class Body>
-VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, Tokens tokens_per_block, Body body) {
+__shared__ uint64_t vm_paged_cost[kWaves + 2];   // waves' sums, then the first sequence and the cost before it
+__shared__ uint32_t vm_paged_last;
+// the step's first kPagedHeld sequences: first row, end row, length
+constexpr uint32_t kPagedHeld = 256;
+__shared__ int32_t vm_paged_seq[3][kPagedHeld];
+
+// Worker w's share: its items' pieces one after another.  tokens_per_block(n, &weight, &align) -> TB;
+// no cut item's align * weight is more than `min_share`; body(job) computes a piece (every thread of the block) and says whether redo(job) has to.
+template <class Tokens, class Body, class Redo>
+VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, uint32_t min_share, Tokens tokens_per_block, Body body,
+                         Redo redo) {
   const VM_K Task& t = task_of(A, ti);
   const PagedDesc D = paged_desc(A, t);
   const uint32_t W = t.p[7], tid = threadIdx.x, g = D.Hq / D.Hkv;
   const VM_G int32_t* cu = gcast<int32_t>(resolve(A, t.p[3]));
   const VM_G int32_t* lens = gcast<int32_t>(resolve(A, t.p[4]));
-  __shared__ uint64_t s_wave[kWaves + 2];
-  __shared__ uint32_t s_last;
-
   auto blocks = [&](const PagedSeq& q) {
     PagedBlocks b;
-    b.tb = tokens_per_block(q.n);
-    b.nb = (q.n + b.tb - 1) / b.tb;
-    b.n = q.n;
-    b.p0 = q.p0;
-    b.len = q.len;
-    b.window = D.window;
+    b.tb = tokens_per_block(q.n, &b.weight, &b.align);
+    b.set(q, D.window);
     return b;
   };
+  auto sequence = [&](uint32_t s, PagedSeq* q) {
+    bool bad;
+    return s < kPagedHeld ? paged_seq(D, uni(vm_paged_seq[0][s]), uni(vm_paged_seq[1][s]), uni(vm_paged_seq[2][s]), q, &bad)
+                          : paged_seq(D, uni(cu[s]), uni(cu[s + 1]), uni(lens[s]), q, &bad);
+  };
+  __syncthreads();                          // a worker before this one has read what it held
   // cost of the thread's sequences, and its sum before them
   const uint32_t per = (D.B + kBlock - 1) / kBlock, first = min(D.B, tid * per), last = min(D.B, first + per);
   uint64_t own = 0;
@@ -170,8 +240,13 @@ VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, Tokens tokens_per_bloc
   for (uint32_t s = first; s < last; ++s) {
     PagedSeq q;
     bool bad;
-    const int32_t c0 = cu[s], c1 = cu[s + 1];
-    if (paged_seq(D, c0, c1, lens[s], &q, &bad)) {
+    const int32_t c0 = cu[s], c1 = cu[s + 1], len = lens[s];
+    if (s < kPagedHeld) {
+      vm_paged_seq[0][s] = c0;
+      vm_paged_seq[1][s] = c1;
+      vm_paged_seq[2][s] = len;
+    }
+    if (paged_seq(D, c0, c1, len, &q, &bad)) {
       const PagedBlocks b = blocks(q);
       own += D.Hkv * b.before(b.nb);
     }
@@ -185,40 +260,48 @@ VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, Tokens tokens_per_bloc
     if ((tid & 63) >= uint32_t(k)) sum += o;
   }
   __syncthreads();
-  if ((tid & 63) == 63) s_wave[tid >> 6] = sum;
+  if ((tid & 63) == 63) vm_paged_cost[tid >> 6] = sum;
   any_bad = __syncthreads_or(any_bad);
   outside = __syncthreads_or(outside);
+  auto uni64 = [](uint64_t x) { return (uint64_t(uni(uint32_t(x >> 32))) << 32) | uni(uint32_t(x)); };
   uint64_t before = sum - own, total = 0;
 #pragma unroll
   for (uint32_t k = 0; k < uint32_t(kWaves); ++k) {
-    if (k < (tid >> 6)) before += s_wave[k];
-    total += s_wave[k];
+    if (k < (tid >> 6)) before += vm_paged_cost[k];
+    total += vm_paged_cost[k];
   }
+  total = uni64(total);
   if (any_bad || outside) paged_zero_rows(A, t, D, w, cu, lens, any_bad);
-  const uint64_t share = max(uint64_t(kMinShare), (total + W - 1) / W);
+  w = uni(w);
+  // a worker's share: share32 << sh, so that positions are divided by it in 32 bits
+  const uint32_t bits = 64 - uint32_t(__builtin_clzll(total | 1)), sh = bits > 31 ? bits - 31 : 0;
+  const uint32_t share32 = uni(max(max(kMinShare, min_share) >> min(sh, 20u), (uint32_t(total >> sh) + W) / W));
+  const uint64_t share = uint64_t(share32) << sh;
   const uint64_t c0 = w * share, c1 = min(total, c0 + share);
   if (c0 >= total) return;
   // the sequence of cost c0
   if (own && before <= c0 && c0 < before + own) {
     uint64_t base = before;
     for (uint32_t s = first; s < last; ++s) {
-      PagedSeq q;
-      bool bad;
-      if (!paged_seq(D, cu[s], cu[s + 1], lens[s], &q, &bad)) continue;
-      const PagedBlocks b = blocks(q);
-      const uint64_t c = D.Hkv * b.before(b.nb);
+      uint64_t c = own;
+      if (per > 1) {
+        PagedSeq q;
+        bool bad;
+        if (!paged_seq(D, cu[s], cu[s + 1], lens[s], &q, &bad)) continue;
+        const PagedBlocks b = blocks(q);
+        c = D.Hkv * b.before(b.nb);
+      }
       if (c0 < base + c) {
-        s_wave[kWaves] = base;
-        s_wave[kWaves + 1] = s;
+        vm_paged_cost[kWaves] = base;
+        vm_paged_cost[kWaves + 1] = s;
         break;
       }
       base += c;
     }
   }
   __syncthreads();
-  auto uni64 = [](uint64_t x) { return (uint64_t(uni(uint32_t(x >> 32))) << 32) | uni(uint32_t(x)); };
-  uint64_t base = uni64(s_wave[kWaves]);
-  uint32_t s = uni(uint32_t(s_wave[kWaves + 1]));
+  uint64_t base = uni64(vm_paged_cost[kWaves]);
+  uint32_t s = uni(uint32_t(vm_paged_cost[kWaves + 1]));
 
   float* scratch = reinterpret_cast<float*>(A->scratch + A->task_scratch[ti]);
   const uint64_t slot_floats = paged_slot_floats(D);
@@ -226,43 +309,47 @@ VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, Tokens tokens_per_bloc
 
   for (; s < D.B && base < c1; ++s) {
     PagedSeq q;
-    bool bad;
-    if (!paged_seq(D, uni(cu[s]), uni(cu[s + 1]), uni(lens[s]), &q, &bad)) continue;
+    if (!sequence(s, &q)) continue;
     const PagedBlocks B = blocks(q);
     const uint64_t S1 = B.before(B.nb);                        // a head's cost
     uint32_t h = 0, b = 0;
+    uint64_t I0 = base;                                        // cost before the item
     if (c0 > base) {
-      const uint64_t x = c0 - base;
-      h = uint32_t(x / S1);
-      const uint64_t rem = x - h * S1;
-      uint32_t lo = 0, hi = B.nb;                              // the last b with before(b) <= rem
-      while (hi - lo > 1) {
-        const uint32_t m = (lo + hi) / 2;
-        if (B.before(m) <= rem) lo = m;
+      while (c0 - I0 >= S1) {                                  // at most Hkv - 1 times
+        I0 += S1;
+        ++h;
+      }
+      uint32_t hi = B.nb;                                      // the last b with before(b) <= c0 - I0
+      while (hi - b > 1) {
+        const uint32_t m = (b + hi) / 2;
+        if (B.before(m) <= c0 - I0) b = m;
         else hi = m;
       }
-      b = lo;
+      I0 += B.before(b);
     }
     for (; h < D.Hkv; ++h, b = 0) {
       bool done = false;
       for (; b < B.nb; ++b) {
-        const uint64_t I0 = base + h * S1 + B.before(b);
         if (I0 >= c1) {
           done = true;
           break;
         }
         const uint32_t ks = B.kstart(b), K = B.kend(b) - ks;
-        const uint64_t I1 = I0 + kItemCost + K;
-        // Keys of the item before worker boundary c: a multiple of kKeyAlign.  The first
-        // piece can be empty (the boundary lies in the item's fixed cost or within
-        // kKeyAlign keys of its start); no other can, since a share is more than kItemCost +
-        // kKeyAlign and the last boundary lies before the item's end.
+        const uint64_t start = I0, I1 = I0 + kItemCost + uint64_t(K) * B.weight;
+        I0 = I1;
+        // Keys of the item before worker boundary c: a multiple of `align`, and none or all of
+        // them where the boundary is nearer than `slack` to the item's start or end, since a
+        // piece has to be worth its partial and the join (3 to 8 us for few rows, about 20
+        // for many; an item of few rows alone takes 10 us and 1.4 per 128 keys).  Boundaries
+        // between give different numbers: a share is at least align * weight.
+        const uint64_t slack = B.weight > 2 || share < 8192 ? 2048 : 512;
+        const uint64_t from = start + kItemCost + slack, to = I1 > slack ? I1 - slack : 0;   // cut in (from, to)
         auto keys_before = [&](uint64_t c) -> uint32_t {
-          if (c <= I0 + kItemCost) return 0;
-          if (c >= I1) return K;
-          return uint32_t(c - I0 - kItemCost) / kKeyAlign * kKeyAlign;
+          if (c <= from) return 0;
+          if (c >= to) return K;
+          return uint32_t((c - start - kItemCost) / B.weight) / B.align * B.align;
         };
-        const uint32_t ka = I0 >= c0 ? 0 : keys_before(c0), kb = I1 <= c1 ? K : keys_before(c1);
+        const uint32_t ka = start >= c0 ? 0 : keys_before(c0), kb = I1 <= c1 ? K : keys_before(c1);
         if (ka >= kb) continue;
         const uint32_t tok0 = b * B.tb;
         PagedJob job;
@@ -274,30 +361,33 @@ VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, Tokens tokens_per_bloc
         job.k0 = ks + ka;
         job.k1 = ks + kb;
         job.part = nullptr;
-        if (ka == 0 && kb == K) {
-          body(job);
-          continue;
+        uint32_t w0 = 0, np = 1;                              // worker of the first piece, pieces
+        if (ka != 0 || kb != K) {
+          // cut by the boundaries v * share in (from, to): w0 + 1, w0 + 2, ...
+          w0 = uint32_t(from >> sh) / share32;
+          while (uint64_t(w0 + 1) * share <= from) ++w0;
+          uint32_t v = uint32_t((to - 1) >> sh) / share32;
+          np = v - w0 + 1;
+          job.part = scratch + (ka ? 2 * uint64_t(w) : 2 * uint64_t(w) + 1) * slot_floats;
         }
-        const uint32_t w0 = uint32_t(I0 / share), w1 = uint32_t((I1 - 1) / share);
-        const uint32_t skip = keys_before((w0 + 1) * share) == 0 ? 1u : 0u;
-        const uint32_t np = w1 - w0 + 1 - skip;
-        job.part = scratch + (w == w0 ? 2 * uint64_t(w) + 1 : 2 * uint64_t(w)) * slot_floats;
-        body(job);
-        // the barrier orders every thread's stores (done: vmcnt 0) before thread 0's
-        // arrival, an agent-scope acquire-release; the last one sees every piece
+        if (body(job)) redo(job);
+        if (!job.part) continue;
+        // The barrier orders every thread's stores (done: vmcnt 0) before thread 0's arrival,
+        // an agent-scope acquire-release that writes this XCD's L2 back, as at the grid
+        // barrier; the last one sees every piece once its caches are invalidated.
         __builtin_amdgcn_s_waitcnt(0x0F70);
         __syncthreads();
         if (tid == 0) {
           const uint32_t n = __hip_atomic_fetch_add(arrivals + w0, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
           if (n == np - 1) __hip_atomic_store(arrivals + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          s_last = n == np - 1;
+          vm_paged_last = n == np - 1;
         }
         __syncthreads();
-        if (s_last) {
+        if (vm_paged_last) {
+          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
           const uint32_t R = job.tokens * g;
           auto slot = [&](uint32_t i) -> const float* {
-            const uint32_t v = w0 + skip + i;
-            return scratch + (v == w0 ? 2 * uint64_t(v) + 1 : 2 * uint64_t(v)) * slot_floats;
+            return scratch + (i ? 2 * uint64_t(w0 + i) : 2 * uint64_t(w0) + 1) * slot_floats;
           };
           auto row_at = [&](uint32_t r) -> uint64_t {
             return (uint64_t(job.row0 + r / g) * D.Hq + h * g + r % g) * D.hd;
@@ -320,7 +410,11 @@ VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, Tokens tokens_per_bloc
 constexpr uint32_t kPagedGenericRows = 32;
 
 template <uint32_t DT, bool Q8>
-VM_DEV void paged_block_generic(Args A, const VM_K Task& t, const PagedDesc& D, const PagedJob& J) {
+VM_LEAF void paged_block_generic(Args A, uint32_t ti, PagedJob J) {
+  A = uargs(A);
+  J.uniform();
+  const VM_K Task& t = task_of(A, ti);
+  const PagedDesc D = paged_desc(A, t);
   const uint32_t lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), g = D.Hq / D.Hkv, hd = D.hd;
   const gbyte* qb = resolve(A, t.a);
   const gbyte* kp = resolve(A, t.b);
@@ -396,12 +490,13 @@ VM_DEV void paged_block_generic(Args A, const VM_K Task& t, const PagedDesc& D, 
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] += __shfl_xor(o[e], msk, 64);
     if (J.part) {
-      if (lane < hd / 8)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) agent_store(J.part + uint64_t(i) * hd + c + e, o[e]);
+      if (lane < hd / 8) {
+        *(v4f*)(J.part + uint64_t(i) * hd + c) = v4f_make(o[0], o[1], o[2], o[3]);
+        *(v4f*)(J.part + uint64_t(i) * hd + c + 4) = v4f_make(o[4], o[5], o[6], o[7]);
+      }
       if (lane == 0) {
-        agent_store(J.part + uint64_t(R) * hd + i, m);
-        agent_store(J.part + uint64_t(R) * (hd + 1) + i, lsum);
+        J.part[uint64_t(R) * hd + i] = m;
+        J.part[uint64_t(R) * (hd + 1) + i] = lsum;
       }
     } else if (lane < hd / 8) {
 #pragma unroll
@@ -423,24 +518,18 @@ VM_TILE void paged_generic(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
   const PagedDesc D = paged_desc(A, t);
   const uint32_t g = D.Hq / D.Hkv;
   for (uint32_t w = lo; w < hi; ++w) {
-    paged_worker(A, ti, w, [&](uint32_t) { return max(1u, kPagedGenericRows / g); },
-                 [&](const PagedJob& J) { paged_block_generic<DT, Q8>(A, t, D, J); });
+    // a wave takes about 2 us for 64 keys of a row, of which a block has up to 32: 0.6 units
+    // a key and row
+    const uint32_t tb = max(1u, kPagedGenericRows / g);
+    auto tokens = [&](uint32_t n, uint32_t* weight, uint32_t* align) {
+      const uint32_t rows = min(tb, n) * g;
+      *weight = min(32u, pow2_at_least(rows));
+      *align = 64;
+      return tb;
+    };
+    paged_worker(A, ti, w, 2048, tokens, [&](const PagedJob& J) { return true; },
+                 [&](const PagedJob& J) { paged_block_generic<DT, Q8>(A, ti, J); });
     __syncthreads();
-  }
-}
-
-VM_DEV void paged_tiles(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
-  const VM_K Task& t = task_of(A, ti);
-  const uint32_t dt = (t.tile_op >> 8) & 0xFF;
-  const bool q8 = uint32_t((aux_of(A) + t.p[6])[PD_CDT]) == DT_I8;
-  if (q8) {
-    if (dt == DT_BF16) paged_generic<DT_BF16, true>(A, ti, lo, hi);
-    else if (dt == DT_F16) paged_generic<DT_F16, true>(A, ti, lo, hi);
-    else paged_generic<DT_F32, true>(A, ti, lo, hi);
-  } else {
-    if (dt == DT_BF16) paged_generic<DT_BF16, false>(A, ti, lo, hi);
-    else if (dt == DT_F16) paged_generic<DT_F16, false>(A, ti, lo, hi);
-    else paged_generic<DT_F32, false>(A, ti, lo, hi);
   }
 }
 

@@ -65,7 +65,7 @@ enum : uint32_t {
 // elements, scale bits, window (0: none)
 enum : uint32_t {
   PD_T = 0, PD_HQ, PD_HKV, PD_HD, PD_PAGE, PD_PAGES, PD_SEQS, PD_MAXP, PD_CDT, PD_ARS, PD_AHS, PD_AOFF, PD_BRS,
-  PD_BHS, PD_BOFF, PD_SCALE, PD_WINDOW, PD_WORDS
+  PD_BHS, PD_BOFF, PD_SCALE, PD_WINDOW, PD_DIVP, PD_DIVG = PD_DIVP + 4, PD_WORDS = PD_DIVG + 4
 };
 // Query heads per kv head, head size, rows per worker's partial block of TOP_PAGED_ATTN at most.
 constexpr uint32_t kPagedMaxGroup = 128;

@@ -454,12 +454,13 @@ struct Checker {
     }
     if (!aux_ok(t.p[6], PD_WORDS)) return fail(ti, "paged cache descriptor");
     const int32_t* d = P.aux.data() + t.p[6];
+    if (d[PD_HQ] < d[PD_HKV]) return fail(ti, "paged cache heads");
     const int64_t T = d[PD_T], Hq = d[PD_HQ], Hkv = d[PD_HKV], hd = d[PD_HD], page = d[PD_PAGE], N = d[PD_PAGES],
                   B = d[PD_SEQS], MP = d[PD_MAXP];
     const uint32_t cdt = uint32_t(d[PD_CDT]);
     if (T < 1 || T >= (1 << 24) || Hkv < 1 || Hkv > (1 << 16) || hd < 8 || hd % 8 || hd > kPagedMaxHd || page < 1 ||
         page > (1 << 16) || N < 1 || B < 1 || MP < 1 || B * MP >= (int64_t(1) << 31) || MP * page >= (int64_t(1) << 31) ||
-        N * Hkv * page >= (int64_t(1) << 40))
+        N > ((int64_t(1) << 32) - 1) / (Hkv * page))
       return fail(ti, "paged cache shape");
     if (!flt(cdt) && cdt != DT_I8) return fail(ti, "paged cache dtype");
     // the pages: a, b of read, dst, p0 of append, b, p0 of attention
@@ -1280,6 +1281,16 @@ static int prepare_program(vmrt_runtime* rt, vmrt_program* lp, const void* bytes
     } else if (top == TOP_DYN_GATHER || top == TOP_DYN_SCATTER) {
       const int32_t rank = P.aux[x];
       for (int d = 0; d < rank; ++d) aux[x + 1 + 3 * rank + d] = int32_t(handle(uint32_t(P.aux[x + 1 + 4 * rank + d])));
+    }
+  }
+  for (const Task& t : P.tasks) {
+    const uint32_t top = t.tile_op & 0xFF;
+    if (top != TOP_CACHE_APPEND && top != TOP_CACHE_READ && top != TOP_PAGED_ATTN) continue;
+    int32_t* d = aux.data() + t.p[6];
+    const DivU32 by[2] = {div_u32(uint32_t(d[PD_PAGE])), div_u32(uint32_t(d[PD_HQ] / d[PD_HKV]))};
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t w[4] = {by[k].d, by[k].m, by[k].s1, by[k].s2};
+      std::memcpy(d + PD_DIVP + 4 * k, w, sizeof w);
     }
   }
   // ---- matmul records, one cache line and more each ----

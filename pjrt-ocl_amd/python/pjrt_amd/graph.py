@@ -705,7 +705,7 @@ class Graph:
             raise GraphError("paged_cache: pages are f32, f16, bf16 or i8")
         if pages < 1 or heads < 1 or page < 1 or head_dim % 8 or not 8 <= head_dim <= 256:
             raise GraphError("paged_cache: at least one page, head and position; head_dim a multiple of 8 up to 256")
-        if page > 1 << 16 or pages >= 1 << 31 or heads > 1 << 16 or pages * heads * page >= 1 << 40:
+        if page > 1 << 16 or pages >= 1 << 31 or heads > 1 << 16 or pages * heads * page >= 1 << 32:
             raise GraphError("paged_cache: too large")
         shape = (pages, heads, page, head_dim)
         k, v = self.state(shape, dt), self.state(shape, dt)
@@ -738,7 +738,7 @@ class Graph:
             raise GraphError(f"{what}: positions of a sequence fit 31 bits")
         ks = cache.k_scale.buf if cache.k_scale is not None else cache.k.buf
         vs = cache.v_scale.buf if cache.v_scale is not None else cache.v.buf
-        return [T, Hq, Hkv, hd, P, N, B, MP, cache.k.dtype, *a, *b, V.f32_bits(scale), window], \
+        return [T, Hq, Hkv, hd, P, N, B, MP, cache.k.dtype, *a, *b, V.f32_bits(scale), window] + [0] * 8, \
             [ks, vs, batch.cu.buf, batch.lens.buf, batch.table.buf]
 
     def cache_append(self, cache: PagedCache, batch: PagedBatch, k: Tensor, v: Tensor) -> None:

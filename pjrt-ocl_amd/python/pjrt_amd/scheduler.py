@@ -510,7 +510,7 @@ def instr_to_task(ins: V.Instr, prog: V.VMProgram, cfg: DeviceConfig) -> V.Task:
         freq, weight, part, workers = prog.aux[ins.aux + 13:ins.aux + 17]
         t = V.Task(V.TOP_ROTARY_GRAD, ins.dst, ins.a, ins.b, ins.imm2, freq, ins.aux, workers, weight, part)
     elif op in V.CACHE_OPS:
-        bufs6 = prog.aux[ins.aux + 17:ins.aux + 23]
+        bufs6 = prog.aux[ins.aux + 25:ins.aux + 31]
         top, p7 = {V.OP_CACHE_APPEND: (V.TOP_CACHE_APPEND, ins.n << 8 | cache_rows_per_tile(ins.n, cfg)),
                    V.OP_CACHE_READ: (V.TOP_CACHE_READ, ins.n << 8 | cache_rows_per_tile(ins.n, cfg)),
                    V.OP_PAGED_ATTN: (V.TOP_PAGED_ATTN, cfg.nlanes)}[op]
@@ -778,9 +778,9 @@ def _instr_reads(ins: V.Instr, prog: V.VMProgram) -> set:
         r = {ins.a, ins.b, ins.imm2, *prog.aux[ins.aux + 13:ins.aux + 15]}
     elif op in V.CACHE_OPS:
         # the pages and scales that append writes keep the rest of what they hold
-        r = {ins.a, ins.b, *prog.aux[ins.aux + 17:ins.aux + 23]}
+        r = {ins.a, ins.b, *prog.aux[ins.aux + 25:ins.aux + 31]}
         if op == V.OP_CACHE_READ:
-            r -= {prog.aux[ins.aux + 17]}
+            r -= {prog.aux[ins.aux + 25]}
         else:
             r |= {ins.dst} if op == V.OP_CACHE_APPEND else set()
     elif op == V.OP_MAP_REGION:
@@ -811,10 +811,10 @@ def _instr_writes(ins: V.Instr, prog: V.VMProgram) -> set:
     if ins.op == V.OP_ROTARY_GRAD:
         return {ins.dst, prog.aux[ins.aux + 15]}
     if ins.op == V.OP_CACHE_APPEND:
-        w = {ins.dst, prog.aux[ins.aux + 17]}
-        return w | set(prog.aux[ins.aux + 18:ins.aux + 20]) if prog.aux[ins.aux + 8] == V.DT_I8 else w
+        w = {ins.dst, prog.aux[ins.aux + 25]}
+        return w | set(prog.aux[ins.aux + 26:ins.aux + 28]) if prog.aux[ins.aux + 8] == V.DT_I8 else w
     if ins.op == V.OP_CACHE_READ:
-        return {ins.dst, prog.aux[ins.aux + 17]}
+        return {ins.dst, prog.aux[ins.aux + 25]}
     return {ins.dst}
 
 
