@@ -33,7 +33,7 @@ namespace vm {
 
 // Costs are in units of about 12.5 ns of one CU: what a key of 128 channels costs a block of
 // 64 rows on the matrix cores, half of what streaming it from HBM costs (all CUs at once).
-constexpr uint32_t kItemCost = 192;        // an item's fixed cost
+constexpr uint32_t kItemCost = 448;        // an item's fixed cost
 constexpr uint32_t kMinShare = 512;        // cost of a worker at least
 
 struct PagedSeq {                          // a sequence with new rows and a place for them
@@ -54,6 +54,7 @@ VM_DEV bool paged_seq(const PagedDesc& D, int32_t c0, int32_t c1, int32_t len, P
 // Blocks of a sequence: key ranges and the cost of the first b blocks of a head.
 struct PagedBlocks {
   uint32_t tb, nb, n, p0, weight, align;   // cut at multiples of `align` keys; weight a power of two
+  uint32_t slack;                          // cost that a piece is worth at least
   int32_t a;                     // kstart(b) = max(0, a + b tb)
   uint32_t i0;                   // the first b with a + b tb > 0
   VM_DEV void set(const PagedSeq& q, uint32_t window) {
@@ -211,8 +212,9 @@ __shared__ uint32_t vm_paged_last;
 constexpr uint32_t kPagedHeld = 256;
 __shared__ int32_t vm_paged_seq[3][kPagedHeld];
 
-// Worker w's share: its items' pieces one after another.  tokens_per_block(n, &weight, &align) -> TB;
-// no cut item's align * weight is more than `min_share`; body(job) computes a piece (every thread of the block) and says whether redo(job) has to.
+// Worker w's share: its items' pieces one after another.  tokens_per_block(n, &blocks) -> TB
+// sets weight, align and slack; align * weight is at most `min_share`; body(job) computes a
+// piece (every thread of the block) and says whether redo(job) has to.
 template <class Tokens, class Body, class Redo>
 VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, uint32_t min_share, Tokens tokens_per_block, Body body,
                          Redo redo) {
@@ -223,7 +225,7 @@ VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, uint32_t min_share, To
   const VM_G int32_t* lens = gcast<int32_t>(resolve(A, t.p[4]));
   auto blocks = [&](const PagedSeq& q) {
     PagedBlocks b;
-    b.tb = tokens_per_block(q.n, &b.weight, &b.align);
+    b.tb = tokens_per_block(q.n, &b);
     b.set(q, D.window);
     return b;
   };
@@ -339,10 +341,12 @@ VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, uint32_t min_share, To
         I0 = I1;
         // Keys of the item before worker boundary c: a multiple of `align`, and none or all of
         // them where the boundary is nearer than `slack` to the item's start or end, since a
-        // piece has to be worth its partial and the join (3 to 8 us for few rows, about 20
-        // for many; an item of few rows alone takes 10 us and 1.4 per 128 keys).  Boundaries
-        // between give different numbers: a share is at least align * weight.
-        const uint64_t slack = B.weight > 2 || share < 8192 ? 2048 : 512;
+        // piece has to be worth its partial and the join (about 8 us for few rows, 20 for
+        // many).  Where lanes are left over anyway (a share of less than 1024) an item of few
+        // rows is cut later: alone it takes 10 us and 1.4 per 128 keys.  The boundaries between
+        // give numbers that differ and are not 0, so that every piece counted below has keys:
+        // a share and the slack are at least align * weight.
+        const uint64_t slack = max(share < 1024 ? max(B.slack, 1024u) : B.slack, B.align * B.weight);
         const uint64_t from = start + kItemCost + slack, to = I1 > slack ? I1 - slack : 0;   // cut in (from, to)
         auto keys_before = [&](uint64_t c) -> uint32_t {
           if (c <= from) return 0;
@@ -521,10 +525,11 @@ VM_TILE void paged_generic(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
     // a wave takes about 2 us for 64 keys of a row, of which a block has up to 32: 0.6 units
     // a key and row
     const uint32_t tb = max(1u, kPagedGenericRows / g);
-    auto tokens = [&](uint32_t n, uint32_t* weight, uint32_t* align) {
+    auto tokens = [&](uint32_t n, PagedBlocks* b) {
       const uint32_t rows = min(tb, n) * g;
-      *weight = min(32u, pow2_at_least(rows));
-      *align = 64;
+      b->weight = min(32u, pow2_at_least(rows));
+      b->align = 64;
+      b->slack = 640;
       return tb;
     };
     paged_worker(A, ti, w, 2048, tokens, [&](const PagedJob& J) { return true; },

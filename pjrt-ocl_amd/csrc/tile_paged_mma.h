@@ -993,15 +993,18 @@ VM_LEAF void paged_mma(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
   const VM_K Task& t = task_of(A, ti);
   const PagedDesc D = paged_desc(A, t);
   const uint32_t g = D.dg.d;
-  // Rows of a block: those with up to 64 rows whole, longer sequences in blocks of 256,
-  // 128 or 64 rows, the most that gives every worker one.
-  const uint32_t share_rows = uint32_t(uint64_t(D.T) * D.Hq / t.p[7]);
-  const uint32_t r = max(share_rows >= 256 ? 256u : share_rows >= 128 ? 128u : 64u, g), long_tb = r / g;
-  const uint32_t long_weight = r > 128 ? 4 : r > 64 ? 2 : 1;
-  auto tokens = [&](uint32_t n, uint32_t* weight, uint32_t* align) {
+  // Rows of a block: sequences of up to 64 rows whole, longer ones in blocks of 256, or of
+  // 128 where those would leave workers without one (512 tokens of 32 heads over 2048: 77 us
+  // in blocks of 128, 94 of 64, 114 of 256).
+  const uint32_t r = max(uint64_t(D.T) * D.Hq >= uint64_t(t.p[7]) * 192 ? 256u : 128u, g), long_tb = r / g;
+  // A key costs about 25 ns in few rows (its share of HBM) and in 128, 41 in 256; half with
+  // heads of 64.
+  const uint32_t unit = HD == 128 ? 2 : 1, long_weight = r > 128 ? 2 * unit : unit;
+  auto tokens = [&](uint32_t n, PagedBlocks* b) {
     const bool few = n * g <= 64;
-    *weight = few ? 2 : long_weight;
-    *align = 256 / *weight;
+    b->weight = few ? unit : long_weight;
+    b->align = r > 128 && !few ? 64 : 128;
+    b->slack = few ? 640 : 1600;
     return few ? n : long_tb;
   };
   for (uint32_t w = lo; w < hi; ++w) {
@@ -1016,32 +1019,6 @@ VM_LEAF void paged_mma(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
     paged_worker(A, ti, w, kMinShare, tokens, body,
                  [&](const PagedJob& J) { paged_block_generic<BF16 ? DT_BF16 : DT_F16, Q8>(A, ti, J); });
     __syncthreads();
-  }
-}
-
-VM_DEV void paged_tiles(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
-  const VM_K Task& t = task_of(A, ti);
-  const VM_K int32_t* d = aux_of(A) + t.p[6];
-  const uint32_t dt = (t.tile_op >> 8) & 0xFF, hd = d[PD_HD];
-  const bool q8 = uint32_t(d[PD_CDT]) == DT_I8;
-  if (dt != DT_F32 && hd <= 128 && !(q8 && hd % 16)) {
-    if (dt == DT_BF16) {
-      if (q8) hd <= 64 ? paged_mma<64, true, true>(A, ti, lo, hi) : paged_mma<128, true, true>(A, ti, lo, hi);
-      else hd <= 64 ? paged_mma<64, true, false>(A, ti, lo, hi) : paged_mma<128, true, false>(A, ti, lo, hi);
-    } else {
-      if (q8) hd <= 64 ? paged_mma<64, false, true>(A, ti, lo, hi) : paged_mma<128, false, true>(A, ti, lo, hi);
-      else hd <= 64 ? paged_mma<64, false, false>(A, ti, lo, hi) : paged_mma<128, false, false>(A, ti, lo, hi);
-    }
-    return;
-  }
-  if (q8) {
-    if (dt == DT_BF16) paged_generic<DT_BF16, true>(A, ti, lo, hi);
-    else if (dt == DT_F16) paged_generic<DT_F16, true>(A, ti, lo, hi);
-    else paged_generic<DT_F32, true>(A, ti, lo, hi);
-  } else {
-    if (dt == DT_BF16) paged_generic<DT_BF16, false>(A, ti, lo, hi);
-    else if (dt == DT_F16) paged_generic<DT_F16, false>(A, ti, lo, hi);
-    else paged_generic<DT_F32, false>(A, ti, lo, hi);
   }
 }
 

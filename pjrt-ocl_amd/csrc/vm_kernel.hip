@@ -21,7 +21,7 @@
 #include "tile_gemv.h"
 #include "tile_index.h"
 #include "tile_mma.h"
-#include "tile_paged_mma.h"
+#include "tile_paged_f32.h"
 #include "tile_reduce.h"
 #include "tile_rotary.h"
 

@@ -266,6 +266,20 @@ ATTEND = [
     ([(70, 200)], 96, 1, 64, 8, "bf16", "bf16", 0, 0),
     ([(1, 2)] * 300, 2, 1, 64, 16, "bf16", "bf16", 0, 0),
     ([(9, 4000)] * 3, 5, 1, 128, 16, "f16", "f16", 0, 1),
+    # f32 on the matrix cores: 16, 32 and 64 rows a block, heads wider than a block, both caches
+    ([(1, 2000), (5, 17), (16, 16), (1, 15)], 6, 2, 64, 16, "f32", "f32", 1, 0),
+    ([(7, 700), (9, 333), (40, 40)], 8, 4, 96, 16, "f32", "f32", 0, 200),
+    ([(1, 5000), (130, 300)], 8, 1, 128, 24, "f32", "f32", 0, 0),
+    ([(1, 3000), (20, 500), (3, 3)], 10, 2, 80, 7, "f32", "i8", 2, 0),
+    ([(33, 700)], 4, 2, 128, 64, "f32", "i8", 0, 333),
+    ([(2, 200)], 70, 1, 64, 16, "f32", "f32", 0, 0),
+    ([(1, 300), (4, 90)], 6, 3, 72, 16, "f32", "i8", 0, 0),
+    ([(1, 300), (4, 90)], 6, 3, 72, 16, "f32", "f32", 0, 0),
+    # items cut into many pieces, on few workers' boundaries and many
+    ([(1, 60000)], 2, 1, 64, 64, "bf16", "bf16", 0, 0),
+    ([(2, 30000), (1, 31000), (1, 5)], 4, 2, 128, 16, "bf16", "i8", 0, 0),
+    ([(100, 20000)], 4, 1, 64, 16, "f16", "f16", 0, 0),
+    ([(1, 20000), (3, 4)], 2, 1, 128, 16, "f32", "f32", 0, 0),
 ]
 
 
@@ -282,7 +296,8 @@ def test_paged_attention(case):
     assert not SU.to_f64(got, dt)[c.cu[-1]:].any()
 
 
-@pytest.mark.parametrize("dt,cache,hd", [("bf16", "bf16", 64), ("f16", "i8", 128), ("f32", "f32", 96), ("bf16", "i8", 64)])
+@pytest.mark.parametrize("dt,cache,hd", [("bf16", "bf16", 64), ("f16", "i8", 128), ("f32", "f32", 96), ("bf16", "i8", 64),
+                                         ("f32", "i8", 128), ("f32", "f32", 136)])
 def test_paged_attention_bad_batches(dt, cache, hd):
     c = SU.Case([(4, 90), (6, 190), (50, 50), (30, 80), (1, 150)], 4, 2, hd, 16, dt, cache, pad=2, seed=7, max_pages=12,
                 first=1)
@@ -297,7 +312,8 @@ def test_paged_attention_bad_batches(dt, cache, hd):
     assert not out[0].any() and not out[c.cu[1]:c.cu[3]].any() and not out[c.cu[4]:].any()
 
 
-@pytest.mark.parametrize("dt,cache,hd", [("bf16", "bf16", 128), ("f16", "f16", 64), ("f32", "f32", 64), ("bf16", "i8", 128)])
+@pytest.mark.parametrize("dt,cache,hd", [("bf16", "bf16", 128), ("f16", "f16", 64), ("f32", "f32", 64), ("bf16", "i8", 128),
+                                         ("f32", "i8", 64), ("f32", "f32", 200)])
 def test_paged_attention_ignores_what_it_does_not_see(dt, cache, hd):
     """NaN and infinities at positions after a row's own and before its window, inside the
     tiles that other rows need: rows that do not see them are as without them."""
@@ -319,7 +335,7 @@ def test_paged_attention_ignores_what_it_does_not_see(dt, cache, hd):
     assert np.isnan(out[39]).any() and not np.isfinite(out[0:5]).all()
 
 
-@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 def test_paged_attention_rising_scores(dt):
     """Scores that grow by hundreds along the keys and ones that are all very low."""
     for sign in (1.0, -1.0):
