@@ -1141,15 +1141,16 @@ class TaskRunner:
         T, H, hd, rot, flags, eps, mag, *st = m.aux_view(t.p[2], 13)
         Z = t.p[3]
         hz = -(-H // Z)
+        units = range(4 * lo, min(4 * hi, T * Z))
         weight = m.load_f(t.b, F32)[:hd] if flags & 2 else None
         pos = m.view(t.p[0], I32)[:T]
         fw = m.view(t.p[1], U32)[:rot].reshape(-1, 2)
-        rows = sorted({u // Z for u in range(4 * lo, min(4 * hi, T * Z))})
+        rows = sorted({u // Z for u in units})
         if not rows:
             return
         y = rotary(self._rows3(t.a, t.adt, st[:3], T, H, hd)[rows], pos[rows], fw, rot, bool(flags & 1), bool(flags & 4),
                    float(_bits_f32(mag & 0xFFFFFFFF)), weight, float(_bits_f32(eps & 0xFFFFFFFF)))
-        for u in range(4 * lo, min(4 * hi, T * Z)):
+        for u in units:
             r, h0 = u // Z, u % Z * hz
             h1 = min(H, h0 + hz)
             if h0 < h1:
@@ -1175,6 +1176,12 @@ class TaskRunner:
             else:
                 dw = np.zeros(hd)
             m.store_f(t.p[5], slice(tile * hd, (tile + 1) * hd), dw, F32)
+            # the worker that arrives last adds the rows up, whichever that is
+            key = (id(t), 0)
+            self.splits[key] = self.splits.get(key, 0) + 1
+            if self.splits[key] == W:
+                del self.splits[key]
+                m.store_f(t.p[6], slice(0, hd), m.load_f(t.p[5], F32)[:W * hd].reshape(W, hd).astype(np.float64).sum(0), F32)
 
     # 24, 25, 26: the paged cache (extension)
     def _paged(self, t):
@@ -1404,8 +1411,8 @@ def _instr_task(prog: Prog, ins, ew_ts: int, mma_t: int):
     elif op == 69:
         top, p = 22, [imm2, prog.aux[aux + 13], aux, 1, n, 0, 0, 0]
     elif op == 70:
-        freq, weight, part, workers = prog.aux[aux + 13:aux + 17]
-        top, p = 23, [imm2, freq, aux, workers, weight, part, 0, 0]
+        freq, weight, part, workers, dw = prog.aux[aux + 13:aux + 18]
+        top, p = 23, [imm2, freq, aux, workers, weight, part, dw, 0]
     elif op in (71, 72, 73):
         top = 24 + op - 71
         p = list(prog.aux[aux + 25:aux + 31]) + [aux, n << 8 | 64 if op < 73 else 1]

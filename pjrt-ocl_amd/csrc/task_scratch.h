@@ -38,6 +38,7 @@ inline uint64_t task_scratch_bytes(const Task& t, uint32_t mma_t) {
     const uint64_t blocks = (uint64_t(t.p[0]) + 63) / 64;
     return (blocks * t.p[4] * 64 + blocks) * 4;
   }
+  if ((t.tile_op & 0xFF) == TOP_ROTARY_GRAD) return 4;      // an arrival counter
   if ((t.tile_op & 0xFF) == TOP_ARGMAX_SEG && t.p[3] > 1) return (2ull * t.p[0] * t.p[3] + t.p[0]) * 4;
   if ((t.tile_op & 0xFF) == TOP_DECODE_ATTN && (t.p[4] >> 16) > 1) {
     const uint64_t H = t.p[4] & 0xFFFF, S = t.p[4] >> 16, hd = t.p[5] & 0xFFFF;

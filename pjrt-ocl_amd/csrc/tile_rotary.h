@@ -14,17 +14,21 @@
 // the quadrant and, as a signed 30-bit fraction, an angle in [-pi/4, pi/4], whose
 // sine and cosine are Taylor sums to x^9 and x^10 (the next terms are below 2^-28).
 //
-// A slot is PW channel pairs (or 2 PW channels that pass): with PW = 8 or 4 it is read
-// and written in 16 / 8 byte runs.  A wave takes one row and the heads of one of
-// its p3 splits: LPH lanes a head (a power of two), 64 / LPH heads at a time, each lane
-// the same slots of every head, so a lane works its sines out once per row.  Both
-// are bound by HBM: x is read and y written once.
+// A slot is PW channel pairs (or 2 PW channels that pass): with PW = 8 or 4 it is read and
+// written in 16 / 8 byte runs.  LPH lanes (a power of two) hold a head, 64 / LPH heads go
+// through a wave at a time, each lane with the same slots of every head.  A wave takes
+// kRotRows rows at a time: their sines go into LDS once (a pair a lane, 35 instructions each; each
+// lane working its own eight pairs out for every row took 48 of 99 us for 8192 rows of 40
+// heads), then the (row, head) pairs pass in batches, the next batch's loads in flight
+// while one is computed (there is one wave per SIMD to hide them).  Both operators are bound
+// by HBM: x is read and y written once.
 #pragma once
 #include "vm_device.h"
 
 namespace vm {
 
-constexpr uint32_t kRotHeads = 4;      // head groups whose loads a wave has in flight at once
+constexpr uint32_t kRotRows = 8;                           // rows of a wave's table of sines at most
+constexpr uint32_t kRotTable = kRotRows * (128 + 8) * 2;   // floats per wave
 
 struct RotDesc {
   uint32_t T, H, hd, rot, flags;
@@ -125,12 +129,14 @@ VM_DEV float head_sum(float x, uint32_t lph) {
   return x;
 }
 
-// The slots of a lane: NS at most (lane, lane + LPH, ...), their channels and sines.
+// The slots of a lane: NS at most (lane, lane + LPH, ...), their channels, weights and places
+// in the table of sines.
 template <int PW, int NS, bool INTER>
 struct RotSlots {
   uint32_t c0[NS], c1[NS];         // first channels of the slot's two runs of PW
+  uint32_t at[NS];                 // its first pair in a row of the table
   bool on[NS];
-  float sn[NS][PW], cs[NS][PW], w0[NS][PW], w1[NS][PW];
+  float w0[NS][PW], w1[NS][PW];
 
   VM_DEV void place(const RotDesc& D, uint32_t l, uint32_t lph) {
     const uint32_t rs = D.rot / (2 * PW), all = D.hd / (2 * PW), R = D.rot / 2;
@@ -142,6 +148,7 @@ struct RotSlots {
       const uint32_t k = min(s, all - 1);
       c0[n] = (!INTER && turn) ? k * PW : k * 2 * PW;
       c1[n] = (!INTER && turn) ? R + k * PW : k * 2 * PW + PW;
+      at[n] = turn ? k * PW : R;   // past the pairs a row of the table has PW turns of 0
     }
   }
   VM_DEV void weights(const VM_G float* w) {
@@ -153,20 +160,13 @@ struct RotSlots {
         w1[n][i] = w[c1[n] + i];
       }
   }
-  // slots that pass get the angle 0 and the magnitude 1; `sign` -1 rotates back
-  VM_DEV void angles(const RotDesc& D, const VM_G uint32_t* freq, int32_t pos, uint32_t l, uint32_t lph, float sign) {
-    const uint32_t rs = D.rot / (2 * PW);
+  // cosine and sine (times the magnitude) of the slot's pairs in the table row
+  VM_DEV void turns(const float* row, int n, float (&cs)[PW], float (&sn)[PW]) const {
+    const float* p = row + 2 * at[n];
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      const uint32_t s = l + n * lph;
-#pragma unroll
-      for (int i = 0; i < PW; ++i) {
-        const uint32_t k = 2 * min(s * PW + i, D.rot / 2 - 1);
-        float a, b;
-        turn_sincos(pos, freq[k], freq[k + 1], &a, &b);
-        sn[n][i] = s < rs ? a * D.mag * sign : 0.0f;
-        cs[n][i] = s < rs ? b * D.mag : 1.0f;
-      }
+    for (int i = 0; i < PW; ++i) {
+      cs[i] = p[2 * i];
+      sn[i] = p[2 * i + 1];
     }
   }
   // element i of run 0 / run 1: with interleaved slots the pair is (2 i, 2 i + 1)
@@ -202,7 +202,71 @@ struct RotSlots {
   }
 };
 
+// The wave's table of the turns of rows [row, row + nr): [nr][R + pw] pairs (cosine, sine)
+// times the magnitude, `sign` -1 to rotate back, and pw turns of 0 at the end of a row.
+VM_DEV void rot_table(const RotDesc& D, float* tab, const VM_G int32_t* pos, const VM_G uint32_t* freq, uint32_t row,
+                      uint32_t nr, uint32_t pw, float sign) {
+  const uint32_t lane = threadIdx.x & 63, R = D.rot / 2, ld = 2 * (R + pw);
+  for (uint32_t i = lane; i < R + pw; i += 64) {
+    const uint32_t k = min(i, R - 1), flo = freq[2 * k], fhi = freq[2 * k + 1];
+    int32_t p[kRotRows];
+#pragma unroll
+    for (uint32_t r = 0; r < kRotRows; ++r) p[r] = pos[min(row + min(r, nr - 1), D.T - 1)];
+#pragma unroll
+    for (uint32_t r = 0; r < kRotRows; ++r) {
+      if (r >= nr) break;
+      float s, c;
+      turn_sincos(p[r], flo, fhi, &s, &c);
+      tab[r * ld + 2 * i] = i < R ? c * D.mag : 1.0f;
+      tab[r * ld + 2 * i + 1] = i < R ? s * D.mag * sign : 0.0f;
+    }
+  }
+  __builtin_amdgcn_wave_barrier();       // the wave's own LDS operations are in order
+}
+
 VM_DEV uint32_t pow2_at_least(uint32_t n) { return n <= 1 ? 1u : 1u << (32 - __builtin_clz(n - 1)); }
+
+// A lane's raw runs of N steps: x, or dy and then x.
+template <uint32_t DT, int PW, int NS, bool GRAD = false>
+struct RotBatch {
+  template <int N>
+  struct X {
+    static constexpr int kN = N;
+    Run<DT, PW> r0[N][NS], r1[N][NS];
+    Run<DT, PW> x0[GRAD ? N : 1][NS], x1[GRAD ? N : 1][NS];
+  };
+};
+
+// Steps 0 .. n / hpw of a wave's (row, head) pairs, 64 / LPH pairs each: whole batches of KB
+// steps (no branch within, so that their chains of latencies overlap), the next one's loads
+// in flight, then the rest one step at a time.  load(first step, batch), compute(first step,
+// batch); before() runs once the first loads are under way.
+template <template <int> class Batch, int KB, class Load, class Compute, class Before>
+VM_DEV void rot_steps(uint32_t n, uint32_t hpw, Load load, Compute compute, Before before) {
+  const uint32_t steps = (n + hpw - 1) / hpw, full = n / hpw / KB;
+  if (full) {
+    Batch<KB> b0, b1;
+    load(0, b0);
+    before();
+    for (uint32_t b = 0; b < full; b += 2) {
+      if (b + 1 < full) load((b + 1) * KB, b1);
+      compute(b * KB, b0);
+      if (b + 1 >= full) break;
+      if (b + 2 < full) load((b + 2) * KB, b0);
+      compute((b + 1) * KB, b1);
+    }
+  }
+  uint32_t s = full * KB;
+  if (s >= steps) return;
+  Batch<1> b;
+  load(s, b);
+  if (!full) before();
+  for (;;) {
+    compute(s, b);
+    if (++s >= steps) break;
+    load(s, b);
+  }
+}
 
 template <uint32_t DT, int PW, int NS, bool INTER>
 VM_DEV void rotary_units(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
@@ -211,7 +275,6 @@ VM_DEV void rotary_units(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
   const uint32_t Z = t.p[3], lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const uint32_t lph = min(64u, pow2_at_least(D.hd / (2 * PW))), hpw = 64 / lph;
   const uint32_t l = lane & (lph - 1), hg = lane / lph;
-  const uint32_t hz = (D.H + Z - 1) / Z;                        // heads of a split
   const gbyte* x = resolve(A, t.a);
   gbyte* y = resolve(A, t.dst);
   const VM_G int32_t* pos = gcast<int32_t>(resolve(A, t.p[0]));
@@ -219,77 +282,100 @@ VM_DEV void rotary_units(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
   const bool norm = D.flags & ROT_NORM;
   const float sign = (D.flags & ROT_INVERSE) ? -1.0f : 1.0f;
   typedef Run<DT, PW> R;
+  constexpr int KB = (DT == DT_F32 ? 2 : 4) / NS;               // a batch's loads: 64 bytes a lane, two in flight
   RotSlots<PW, NS, INTER> S;
   S.place(D, l, lph);
   if (norm) S.weights(gcast<float>(resolve(A, t.b)));
   const float inv_hd = 1.0f / float(D.hd);
-  for (uint32_t tile = lo; tile < hi; ++tile) {
-    const uint32_t u = 4 * tile + wave;
-    if (u >= D.T * Z) break;
-    const uint32_t row = u / Z, h0 = (u % Z) * hz, h1 = min(D.H, h0 + hz);
-    if (h0 >= h1) continue;
-    S.angles(D, freq, pos[row], l, lph, sign);
-    const uint64_t xr = uint64_t(row) * D.ars + D.aoff, yr = uint64_t(row) * D.H * D.hd;
-    for (uint32_t hb = h0; hb < h1; hb += hpw * kRotHeads) {
-      R r0[kRotHeads][NS], r1[kRotHeads][NS];
+  float* tab = lds_ptr<float>() + wave * kRotTable;
+  const uint32_t ld = 2 * (D.rot / 2 + PW);
+  // rows [row, row + nr), heads [h0, h1)
+  auto unit = [&](uint32_t row, uint32_t nr, uint32_t h0, uint32_t h1) {
+    const uint32_t nh = h1 - h0, n = nr * nh;
+    // pair `s hpw + hg`: the lane's row (of the unit) and head; past the last it is the last
+    auto which = [&](uint32_t s, uint32_t* r, uint32_t* h) {
+      const uint32_t p = min(s * hpw + hg, n - 1);
+      *r = p / nh;
+      *h = h0 + p - *r * nh;
+    };
+    auto load = [&](uint32_t s0, auto& B) {
 #pragma unroll
-      for (uint32_t k = 0; k < kRotHeads; ++k)
-        if (hb + k * hpw < h1) {
-          const uint32_t h = min(hb + k * hpw + hg, h1 - 1);
+      for (int k = 0; k < B.kN; ++k) {
+        uint32_t r, h;
+        which(s0 + k, &r, &h);
+        const uint64_t e = uint64_t(row + r) * D.ars + uint64_t(h) * D.ahs + D.aoff;
 #pragma unroll
-          for (int n = 0; n < NS; ++n) {
-            r0[k][n].load(x, xr + uint64_t(h) * D.ahs + S.c0[n]);
-            r1[k][n].load(x, xr + uint64_t(h) * D.ahs + S.c1[n]);
-          }
+        for (int s = 0; s < NS; ++s) {
+          B.r0[k][s].load(x, e + S.c0[s]);
+          B.r1[k][s].load(x, e + S.c1[s]);
         }
+      }
+    };
+    auto compute = [&](uint32_t s0, const auto& B) {
 #pragma unroll
-      for (uint32_t k = 0; k < kRotHeads; ++k) {
-        if (hb + k * hpw >= h1) break;
-        const uint32_t h = hb + k * hpw + hg;
-        float r = 1.0f;
+      for (int k = 0; k < B.kN; ++k) {
+        uint32_t r, h;
+        which(s0 + k, &r, &h);
+        const bool in = (s0 + k) * hpw + hg < n;
+        float z = 1.0f;
         if (norm) {
           float ss = 0.0f;
 #pragma unroll
-          for (int n = 0; n < NS; ++n)
-            if (S.on[n])
+          for (int s = 0; s < NS; ++s)
 #pragma unroll
-              for (int i = 0; i < PW; ++i) {
-                const float a = r0[k][n].get(i), b = r1[k][n].get(i);
-                ss = fmaf(a, a, fmaf(b, b, ss));
-              }
-          r = 1.0f / sqrtf(fmaf(head_sum(ss, lph), inv_hd, D.eps));
+            for (int i = 0; i < PW; ++i) {
+              const float a = S.on[s] ? B.r0[k][s].get(i) : 0.0f, c = S.on[s] ? B.r1[k][s].get(i) : 0.0f;
+              ss = fmaf(a, a, fmaf(c, c, ss));
+            }
+          z = 1.0f / sqrtf(fmaf(head_sum(ss, lph), inv_hd, D.eps));
         }
+        const uint64_t e = (uint64_t(row + r) * D.H + h) * D.hd;
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          float f0[PW], f1[PW];
+        for (int s = 0; s < NS; ++s) {
+          float f0[PW], f1[PW], cs[PW], sn[PW];
+          S.turns(tab + r * ld, s, cs, sn);
 #pragma unroll
           for (int i = 0; i < PW; ++i) {
-            float a, b;
-            S.pair(r0[k][n], r1[k][n], i, &a, &b);
+            float a, c;
+            S.pair(B.r0[k][s], B.r1[k][s], i, &a, &c);
             if (norm) {
               float wa, wb;
-              S.weight_pair(n, i, &wa, &wb);
-              a = a * r * wa;
-              b = b * r * wb;
+              S.weight_pair(s, i, &wa, &wb);
+              a = a * z * wa;
+              c = c * z * wb;
             }
-            S.unpair(f0, f1, i, a * S.cs[n][i] - b * S.sn[n][i], b * S.cs[n][i] + a * S.sn[n][i]);
+            S.unpair(f0, f1, i, a * cs[i] - c * sn[i], c * cs[i] + a * sn[i]);
           }
-          if (S.on[n] && h < h1) {
-            R o0, o1;
-            o0.put(f0);
-            o1.put(f1);
-            o0.store(y, yr + uint64_t(h) * D.hd + S.c0[n]);
-            o1.store(y, yr + uint64_t(h) * D.hd + S.c1[n]);
+          R o0, o1;
+          o0.put(f0);
+          o1.put(f1);
+          if (S.on[s] && in) {
+            o0.store(y, e + S.c0[s]);
+            o1.store(y, e + S.c1[s]);
           }
         }
       }
-    }
+    };
+    rot_steps<RotBatch<DT, PW, NS>::template X, KB>(n, hpw, load, compute,
+                                                    [&] { rot_table(D, tab, pos, freq, row, nr, PW, sign); });
+  };
+  if (Z == 1) {
+    // tile: four rows; a wave's quarter of the entry's rows, kRotRows at a time
+    const uint32_t r0 = 4 * lo, rows = min(D.T, 4 * hi) - r0;
+    uint32_t r = r0 + rows * wave / 4;
+    const uint32_t end = r0 + rows * (wave + 1) / 4;
+    for (; r < end; r += kRotRows) unit(r, min(kRotRows, end - r), 0, D.H);
+    return;
   }
+  const uint32_t hz = (D.H + Z - 1) / Z;                        // heads of a split
+  for (uint32_t u = 4 * lo + wave; u < min(4 * hi, D.T * Z); u += 4)
+    if (u % Z * hz < D.H) unit(u / Z, 1, u % Z * hz, min(D.H, u % Z * hz + hz));
 }
 
-// Worker `tile` of p3: rows and heads in (row, head group) order, a contiguous share
-// of them, with the lane's part of dweight in registers until the end; then the head
-// groups of a wave and the four waves are added in LDS, in a fixed order.
+// Worker `tile` of p3: a contiguous share of the (row, head) pairs, a quarter of it a wave,
+// with the lane's part of dweight in registers until the end; then the head groups of a
+// wave and the four waves are added in LDS and left in p5, and the worker that arrives
+// last adds the workers' rows into p6, all in an order of their own.
 template <uint32_t DT, int PW, int NS, bool INTER>
 VM_DEV void rotary_grad_worker(Args A, uint32_t ti, uint32_t tile) {
   const VM_K Task& t = task_of(A, ti);
@@ -303,90 +389,99 @@ VM_DEV void rotary_grad_worker(Args A, uint32_t ti, uint32_t tile) {
   const VM_G int32_t* pos = gcast<int32_t>(resolve(A, t.p[0]));
   const VM_G uint32_t* freq = gcast<uint32_t>(resolve(A, t.p[1]));
   typedef Run<DT, PW> R;
+  constexpr int KB = DT == DT_F32 || NS > 1 ? 1 : 2;
   RotSlots<PW, NS, INTER> S;
   S.place(D, l, lph);
   S.weights(gcast<float>(resolve(A, t.p[4])));
-  float g0[NS][PW], g1[NS][PW];                    // dweight of run 0 / run 1
+  float g0[NS][PW], g1[NS][PW];                    // dweight of the pair's first / second channel
 #pragma unroll
   for (int n = 0; n < NS; ++n)
 #pragma unroll
     for (int i = 0; i < PW; ++i) g0[n][i] = g1[n][i] = 0.0f;
   const float inv_hd = 1.0f / float(D.hd);
-  // rows [t0, t1) of the worker, its waves every fourth
-  const uint32_t t0 = uint32_t(uint64_t(D.T) * D.H * tile / W), t1 = uint32_t(uint64_t(D.T) * D.H * (tile + 1) / W);
-  // (row, head) pairs t0 .. t1 - 1: the waves take runs of them that share a row
-  uint32_t at = t0, turn = 0;
-  while (at < t1) {
-    const uint32_t row = at / D.H, h0 = at % D.H, h1 = min(D.H, h0 + (t1 - at));
-    at += h1 - h0;
-    // a row's heads go to the waves in blocks of hpw * 2
-    const uint32_t blk = hpw * 2, nblk = (h1 - h0 + blk - 1) / blk;
-    bool have = false;
-    for (uint32_t b = 0; b < nblk; ++b, turn = (turn + 1) & 3) {
-      if (turn != wave) continue;
-      if (!have) S.angles(D, freq, pos[row], l, lph, -1.0f);
-      have = true;
-      R y0[2][NS], y1[2][NS], x0[2][NS], x1[2][NS];
+  float* tab = lds_ptr<float>() + wave * kRotTable;
+  const uint32_t ld = 2 * (D.rot / 2 + PW), H = D.H;
+  const uint64_t all = uint64_t(D.T) * H;
+  const uint32_t t0 = uint32_t(all * tile / W), t1 = uint32_t(all * (tile + 1) / W);
+  uint32_t at = t0 + uint32_t(uint64_t(t1 - t0) * wave / 4);
+  const uint32_t end = t0 + uint32_t(uint64_t(t1 - t0) * (wave + 1) / 4);
+  while (at < end) {
+    const uint32_t row = at / H, last = uint32_t(min(uint64_t(end), uint64_t(row + kRotRows) * H));
+    const uint32_t first = at - row * H, n = last - at;         // pairs `first` .. of the rows from `row`
+    at = last;
+    auto which = [&](uint32_t s, uint32_t* r, uint32_t* h) {
+      const uint32_t p = first + min(s * hpw + hg, n - 1);
+      *r = p / H;
+      *h = p - *r * H;
+    };
+    auto load = [&](uint32_t s0, auto& B) {
 #pragma unroll
-      for (uint32_t k = 0; k < 2; ++k) {
-        const uint32_t h = min(h0 + b * blk + k * hpw + hg, h1 - 1);
-        const uint64_t ye = uint64_t(row) * D.ars + uint64_t(h) * D.ahs + D.aoff;
-        const uint64_t xe = uint64_t(row) * D.brs + uint64_t(h) * D.bhs + D.boff;
+      for (int k = 0; k < B.kN; ++k) {
+        uint32_t r, h;
+        which(s0 + k, &r, &h);
+        const uint64_t ye = uint64_t(row + r) * D.ars + uint64_t(h) * D.ahs + D.aoff;
+        const uint64_t xe = uint64_t(row + r) * D.brs + uint64_t(h) * D.bhs + D.boff;
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          y0[k][n].load(dy, ye + S.c0[n]);
-          y1[k][n].load(dy, ye + S.c1[n]);
-          x0[k][n].load(x, xe + S.c0[n]);
-          x1[k][n].load(x, xe + S.c1[n]);
+        for (int s = 0; s < NS; ++s) {
+          B.r0[k][s].load(dy, ye + S.c0[s]);
+          B.r1[k][s].load(dy, ye + S.c1[s]);
+          B.x0[k][s].load(x, xe + S.c0[s]);
+          B.x1[k][s].load(x, xe + S.c1[s]);
         }
       }
+    };
+    auto compute = [&](uint32_t s0, const auto& B) {
 #pragma unroll
-      for (uint32_t k = 0; k < 2; ++k) {
-        const uint32_t h = h0 + b * blk + k * hpw + hg;
-        const bool in = h < h1;
+      for (int k = 0; k < B.kN; ++k) {
+        uint32_t r, h;
+        which(s0 + k, &r, &h);
+        const bool in = (s0 + k) * hpw + hg < n;
         float ss = 0.0f, dot = 0.0f;
         float za[NS][PW], zb[NS][PW], xa[NS][PW], xb[NS][PW];
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
+        for (int s = 0; s < NS; ++s) {
+          float cs[PW], sn[PW];
+          S.turns(tab + r * ld, s, cs, sn);
 #pragma unroll
           for (int i = 0; i < PW; ++i) {
-            float a, b2, wa, wb;
-            S.pair(y0[k][n], y1[k][n], i, &a, &b2);
-            S.pair(x0[k][n], x1[k][n], i, &xa[n][i], &xb[n][i]);
-            S.weight_pair(n, i, &wa, &wb);
-            za[n][i] = a * S.cs[n][i] - b2 * S.sn[n][i];
-            zb[n][i] = b2 * S.cs[n][i] + a * S.sn[n][i];
-            if (S.on[n]) {
-              ss = fmaf(xa[n][i], xa[n][i], fmaf(xb[n][i], xb[n][i], ss));
-              dot = fmaf(za[n][i] * wa, xa[n][i], fmaf(zb[n][i] * wb, xb[n][i], dot));
-            }
+            float a, c, wa, wb;
+            S.pair(B.r0[k][s], B.r1[k][s], i, &a, &c);
+            S.pair(B.x0[k][s], B.x1[k][s], i, &xa[s][i], &xb[s][i]);
+            xa[s][i] = S.on[s] ? xa[s][i] : 0.0f;
+            xb[s][i] = S.on[s] ? xb[s][i] : 0.0f;
+            S.weight_pair(s, i, &wa, &wb);
+            za[s][i] = a * cs[i] - c * sn[i];
+            zb[s][i] = c * cs[i] + a * sn[i];
+            ss = fmaf(xa[s][i], xa[s][i], fmaf(xb[s][i], xb[s][i], ss));
+            dot = fmaf(za[s][i] * wa, xa[s][i], fmaf(zb[s][i] * wb, xb[s][i], dot));
           }
-        const float r = 1.0f / sqrtf(fmaf(head_sum(ss, lph), inv_hd, D.eps));
-        const float c = r * r * r * (head_sum(dot, lph) * inv_hd);
+        }
+        const float z = 1.0f / sqrtf(fmaf(head_sum(ss, lph), inv_hd, D.eps));
+        const float c = z * z * z * (head_sum(dot, lph) * inv_hd);
+        const uint64_t e = (uint64_t(row + r) * H + h) * D.hd;
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
+        for (int s = 0; s < NS; ++s) {
           float f0[PW], f1[PW];
 #pragma unroll
           for (int i = 0; i < PW; ++i) {
             float wa, wb;
-            S.weight_pair(n, i, &wa, &wb);
-            S.unpair(f0, f1, i, r * wa * za[n][i] - xa[n][i] * c, r * wb * zb[n][i] - xb[n][i] * c);
-            if (in) {
-              g0[n][i] = fmaf(za[n][i] * r, xa[n][i], g0[n][i]);
-              g1[n][i] = fmaf(zb[n][i] * r, xb[n][i], g1[n][i]);
-            }
+            S.weight_pair(s, i, &wa, &wb);
+            S.unpair(f0, f1, i, z * wa * za[s][i] - xa[s][i] * c, z * wb * zb[s][i] - xb[s][i] * c);
+            g0[s][i] = in ? fmaf(za[s][i] * z, xa[s][i], g0[s][i]) : g0[s][i];
+            g1[s][i] = in ? fmaf(zb[s][i] * z, xb[s][i], g1[s][i]) : g1[s][i];
           }
-          if (S.on[n] && in) {
-            R o0, o1;
-            o0.put(f0);
-            o1.put(f1);
-            const uint64_t e = (uint64_t(row) * D.H + h) * D.hd;
-            o0.store(dx, e + S.c0[n]);
-            o1.store(dx, e + S.c1[n]);
+          R o0, o1;
+          o0.put(f0);
+          o1.put(f1);
+          if (S.on[s] && in) {
+            o0.store(dx, e + S.c0[s]);
+            o1.store(dx, e + S.c1[s]);
           }
         }
       }
-    }
+    };
+    rot_steps<RotBatch<DT, PW, NS, true>::template X, KB>(
+        n, hpw, load, compute, [&] { rot_table(D, tab, pos, freq, row, min(kRotRows, D.T - row), PW, -1.0f); });
   }
   // [4 hpw][hd] partial rows in LDS: hpw * hd <= 64 * 2 PW, so at most 16 KiB.  The
   // sums are by pair: element i of g0 belongs to channel c0 + i, or c0 + 2 i interleaved
@@ -408,11 +503,55 @@ VM_DEV void rotary_grad_worker(Args A, uint32_t ti, uint32_t tile) {
       }
     }
   __syncthreads();
-  VM_G float* part = gcast<float>(resolve(A, t.p[5])) + uint64_t(tile) * D.hd;
+  VM_G float* part = gcast<float>(resolve(A, t.p[5]));
   for (uint32_t d = threadIdx.x; d < D.hd; d += kBlock) {
     float s = 0.0f;
     for (uint32_t k = 0; k < 4 * hpw; ++k) s += lds[k * D.hd + d];
-    part[d] = s;
+    part[uint64_t(tile) * D.hd + d] = s;
+  }
+  // the barrier orders every thread's stores (done: vmcnt 0) before thread 0's arrival, an
+  // agent-scope acquire-release that writes this XCD's L2 back
+  uint32_t* arrivals = reinterpret_cast<uint32_t*>(A->scratch + A->task_scratch[ti]);
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  __syncthreads();
+  uint32_t* flag = reinterpret_cast<uint32_t*>(lds);
+  if (threadIdx.x == 0) {
+    const uint32_t before = __hip_atomic_fetch_add(arrivals, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    if (before == W - 1) __hip_atomic_store(arrivals, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = before == W - 1;
+  }
+  __syncthreads();
+  const bool sum = *flag;
+  __syncthreads();
+  if (!sum) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  // pairs of channels by runs of rows: thread (c, run) adds rows run, run + runs, ...
+  const uint32_t half = D.hd / 2, runs = kBlock / pow2_at_least(half), c = threadIdx.x % half, run = threadIdx.x / half;
+  float* acc = lds;                                  // [runs][hd]
+  if (run < runs) {
+    float a = 0.0f, b = 0.0f;
+    constexpr uint32_t U = 16;
+    for (uint32_t k0 = run; k0 < W; k0 += U * runs) {
+      f32x2_t v[U];
+#pragma unroll
+      for (uint32_t k = 0; k < U; ++k)
+        v[k] = *(const VM_G f32x2_t*)(part + uint64_t(min(k0 + k * runs, W - 1)) * D.hd + 2 * c);
+#pragma unroll
+      for (uint32_t k = 0; k < U; ++k)
+        if (k0 + k * runs < W) {
+          a += v[k].x;
+          b += v[k].y;
+        }
+    }
+    acc[run * D.hd + 2 * c] = a;
+    acc[run * D.hd + 2 * c + 1] = b;
+  }
+  __syncthreads();
+  VM_G float* dw = gcast<float>(resolve(A, t.p[6]));
+  for (uint32_t d = threadIdx.x; d < D.hd; d += kBlock) {
+    float s = 0.0f;
+    for (uint32_t k = 0; k < runs; ++k) s += acc[k * D.hd + d];
+    dw[d] = s;
   }
 }
 

@@ -449,7 +449,7 @@ struct Checker {
       }
       if (t.p[3] < 1 || t.p[3] > 4096) return fail(ti, "rotary gradient workers");
       if (!rows_ok(t.b, adt, d + RD_BRS, T, H, hd)) return fail(ti, "rotary gradient's rows");
-      return (has(t.p[4], hd, DT_F32) && has(t.p[5], uint64_t(t.p[3]) * hd, DT_F32)) ||
+      return (has(t.p[4], hd, DT_F32) && has(t.p[5], uint64_t(t.p[3]) * hd, DT_F32) && has(t.p[6], hd, DT_F32)) ||
              fail(ti, "rotary gradient's weight");
     }
     if (!aux_ok(t.p[6], PD_WORDS)) return fail(ti, "paged cache descriptor");
@@ -1266,7 +1266,7 @@ static int prepare_program(vmrt_runtime* rt, vmrt_program* lp, const void* bytes
     if (top == TOP_ROTARY || top == TOP_ROTARY_GRAD)
       for (int k = 0; k < 2; ++k) t.p[k] = handle(orig.p[k]);
     if (top == TOP_ROTARY_GRAD)
-      for (int k = 4; k < 6; ++k) t.p[k] = handle(orig.p[k]);
+      for (int k = 4; k < 7; ++k) t.p[k] = handle(orig.p[k]);
     if (top == TOP_CACHE_APPEND || top == TOP_CACHE_READ || top == TOP_PAGED_ATTN)
       for (int k = 0; k < 6; ++k) t.p[k] = handle(orig.p[k]);
   }

@@ -688,12 +688,12 @@ class Graph:
         flags = interleaved * V.ROT_INTERLEAVED | V.ROT_NORM
         dst = self._new(x.shape, dt)
         workers = rotary_grad_workers(T, H)
-        part = self._new((workers, hd), V.DT_F32)
+        part, dw = self._new((workers, hd), V.DT_F32), self._new((hd,), V.DT_F32)
         desc = self.add_aux([T, H, hd, rot, flags, V.f32_bits(eps), V.f32_bits(magnitude), drs, dhs, doff,
-                             xrs, xhs, xoff, freq.buf, weight.buf, part.buf, workers])
+                             xrs, xhs, xoff, freq.buf, weight.buf, part.buf, workers, dw.buf])
         self.emit(V.Instr(V.OP_ROTARY_GRAD, dst=dst.buf, a=db, b=xb, n=T, imm=H, aux=desc, imm2=pos.buf,
                           reads_hint=(pos.buf, freq.buf, weight.buf)))
-        return dst, self.reduce_axis(part, 0, V.RED_SUM)
+        return dst, dw
 
     def paged_cache(self, pages: int, heads: int, page: int, head_dim: int, dtype="bf16") -> PagedCache:
         """State inputs of a cache of ``pages`` pages of ``page`` positions: k and v

@@ -297,8 +297,8 @@ def red_splits(n_out: int, red: int, dt: int, cfg: DeviceConfig) -> int:
 
 
 def rotary_splits(T: int, H: int, cfg: DeviceConfig) -> int:
-    """Head splits of a TOP_ROTARY row (p3): a wave takes a row's heads of one split, so
-    few rows are cut until every wave of the lanes has work or a split is four heads."""
+    """Head splits of a TOP_ROTARY row (p3): few rows are cut by heads until every wave of
+    the lanes has work or a split is four heads."""
     z = 1
     while T * z * 2 <= 4 * cfg.nlanes and H >= 8 * z:
         z *= 2
@@ -507,8 +507,8 @@ def instr_to_task(ins: V.Instr, prog: V.VMProgram, cfg: DeviceConfig) -> V.Task:
         t = V.Task(V.TOP_ROTARY, ins.dst, ins.a, ins.b, ins.imm2, freq, ins.aux,
                    rotary_splits(ins.n, ins.imm, cfg), ins.n)
     elif op == V.OP_ROTARY_GRAD:
-        freq, weight, part, workers = prog.aux[ins.aux + 13:ins.aux + 17]
-        t = V.Task(V.TOP_ROTARY_GRAD, ins.dst, ins.a, ins.b, ins.imm2, freq, ins.aux, workers, weight, part)
+        freq, weight, part, workers, dw = prog.aux[ins.aux + 13:ins.aux + 18]
+        t = V.Task(V.TOP_ROTARY_GRAD, ins.dst, ins.a, ins.b, ins.imm2, freq, ins.aux, workers, weight, part, dw)
     elif op in V.CACHE_OPS:
         bufs6 = prog.aux[ins.aux + 25:ins.aux + 31]
         top, p7 = {V.OP_CACHE_APPEND: (V.TOP_CACHE_APPEND, ins.n << 8 | cache_rows_per_tile(ins.n, cfg)),
@@ -809,7 +809,7 @@ def _instr_writes(ins: V.Instr, prog: V.VMProgram) -> set:
     if ins.op == V.OP_ARGMAX_SEG:
         return {ins.dst, ins.b}
     if ins.op == V.OP_ROTARY_GRAD:
-        return {ins.dst, prog.aux[ins.aux + 15]}
+        return {ins.dst, prog.aux[ins.aux + 15], prog.aux[ins.aux + 17]}
     if ins.op == V.OP_CACHE_APPEND:
         w = {ins.dst, prog.aux[ins.aux + 25]}
         return w | set(prog.aux[ins.aux + 26:ins.aux + 28]) if prog.aux[ins.aux + 8] == V.DT_I8 else w
@@ -1209,9 +1209,19 @@ class _Scheduler:
         shaped, maps = [], []
         for i in sorted(indices):
             (maps if self.task(i).tile_op == V.TOP_EW else shaped).append(i)
-        units = []
+        units, rotary = [], {}
         for i in shaped:
             t = self.task(i)
+            if t.tile_op == V.TOP_ROTARY:
+                # queries and keys of the same rows: each lane takes its share of both, so
+                # that they end together (8192 rows of 32 and 8 heads: 75 us in chunks of
+                # their own, with 2 of 256 tiles on a third of the lanes)
+                tiles, cost = n_tiles(t, self.cfg), task_cost(t, self.cfg, self.prog)
+                if tiles in rotary:
+                    u = rotary[tiles]
+                    units[u] = (units[u][0] + [self.task_id(i)], tiles, units[u][2] + cost, 1, False)
+                    continue
+                rotary[tiles] = len(units)
             units.append(([self.task_id(i)], n_tiles(t, self.cfg),
                           task_cost(t, self.cfg, self.prog),
                           _tile_quantum(t, self.cfg, self.prog),

@@ -66,8 +66,9 @@ which does not use them is byte-for-byte a reference program):
   rotary positions of the heads of [T, H, hd] rows, with an optional RMS norm of
   each head before.  Task: a x (gradient: a dy, b x), b weight (gradient: p4), p0
   positions, p1 frequencies (u32 pairs, 64-bit fixed-point turns per position), p2
-  descriptor (``RD_*`` words of vm_abi.h), p3 head splits Z; tile = four (row, split)
-  pairs.  Gradient: p3 workers, p5 partial sums of dweight [p3, hd]; tile = worker.
+  descriptor (``RD_*`` words of vm_abi.h), p3 head splits Z of a
+  row, p4 rows; tile = four (row, split) pairs.  Gradient: p3 workers, p5 partial sums of dweight
+  [p3, hd], p6 dweight, which the last worker adds up; tile = worker.
 * ``OP_CACHE_APPEND`` (71), ``OP_CACHE_READ`` (72), ``OP_PAGED_ATTN`` (73) / tile ops
   24, 25, 26: new rows into the pages of a cache, the rows of a batch back out of
   it, and attention over it.  Instr: aux -> the descriptor (``PD_*`` words), then
