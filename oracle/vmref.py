@@ -593,13 +593,13 @@ def rotary_grad(dy, x, pos, freq_words, rot, interleaved, mag, weight, eps):
 
 
 def paged_rows(T, cu, lens, table, n_pages, page):
-    """[(row, sequence, position)] of the rows that belong to a sequence whose length
-    fits them and its pages."""
+    """[(row, sequence, position)] of the rows that belong to a sequence all of whose
+    rows are the step's and whose length fits them and its pages."""
     out = []
     for s in range(len(lens)):
-        a, b = (min(max(int(c), 0), T) for c in cu[s:s + 2])
+        a, b = int(cu[s]), int(cu[s + 1])
         n, length = b - a, int(lens[s])
-        if n > 0 and n <= length <= table.shape[1] * page:
+        if a >= 0 and b <= T and 0 < n <= length <= table.shape[1] * page:
             out += [(a + i, s, length - n + i) for i in range(n)]
     return out
 

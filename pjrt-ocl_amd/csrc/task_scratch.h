@@ -47,13 +47,13 @@ inline uint64_t task_scratch_bytes(const Task& t, uint32_t mma_t) {
   return 0;
 }
 
-// Scratch of a paged attention task (tile_paged.h): two partial slots per worker and an
-// arrival counter each.  `aux`: the program's aux words.
+// Scratch of a paged attention task (tile_paged.h): kMaxLanes arrival counters and two
+// partial slots per worker.  `aux`: the program's aux words.
 inline uint64_t paged_scratch_bytes(const Task& t, const int32_t* aux) {
   const int32_t* d = aux + t.p[6];
   const uint64_t rows = std::min<uint64_t>(kPagedMaxRows, uint64_t(d[PD_T]) * (d[PD_HQ] / d[PD_HKV]));
   const uint64_t slot = (rows * (uint64_t(d[PD_HD]) + 2) + 3) & ~uint64_t(3);
-  return (2 * slot + 1) * t.p[7] * 4;
+  return (kMaxLanes + 2 * slot * t.p[7]) * 4;
 }
 
 }  // namespace vm

@@ -22,9 +22,10 @@
 // order.  So one long sequence and many short ones keep every CU as busy, the result
 // depends on the lengths alone, and nothing waits.
 //
-// Scratch: 2 W slots of kPagedMaxRows' (or T g) rows x (hd + 2) floats: worker w's piece of
-// an item that begins before it in slot 2 w, of one that ends after it in 2 w + 1; then W
-// arrival counters, by the worker of the item's first piece.
+// Scratch: kMaxLanes arrival counters, by the worker of the item's first piece, 0 between
+// tasks (tasks that share the scratch have partials of other sizes, so the counters come
+// first); then 2 W slots of kPagedMaxRows' (or T g) rows x (hd + 2) floats: worker w's piece
+// of an item that begins before it in slot 2 w, of one that ends after it in 2 w + 1.
 #pragma once
 #include "tile_attn.h"
 #include "tile_cache.h"
@@ -39,15 +40,15 @@ constexpr uint32_t kMinShare = 512;        // cost of a worker at least
 struct PagedSeq {                          // a sequence with new rows and a place for them
   uint32_t r0, n, len, p0;                 // first row, rows, length, first row's position
 };
-// Sequence s, false when it has no rows or its length does not fit them; `bad`: it has
-// rows that must be 0.
+// Sequence s, false when it has no rows of the step, some of its rows are not the step's or its
+// length does not fit them; `bad`: it has rows that must be 0.
 VM_DEV bool paged_seq(const PagedDesc& D, int32_t c0, int32_t c1, int32_t len, PagedSeq* q, bool* bad) {
   const uint32_t a = uint32_t(min(max(c0, 0), int32_t(D.T))), b = uint32_t(min(max(c1, 0), int32_t(D.T)));
   q->r0 = a;
   q->n = b > a ? b - a : 0;
   q->len = uint32_t(len);
   q->p0 = uint32_t(len) - q->n;
-  *bad = q->n && (len < int32_t(q->n) || uint32_t(len) > D.MP * D.P);
+  *bad = q->n && (c0 < 0 || c1 > int32_t(D.T) || len < int32_t(q->n) || uint32_t(len) > D.MP * D.P);
   return q->n && !*bad;
 }
 
@@ -305,9 +306,9 @@ VM_DEV void paged_worker(Args A, uint32_t ti, uint32_t w, uint32_t min_share, To
   uint64_t base = uni64(vm_paged_cost[kWaves]);
   uint32_t s = uni(uint32_t(vm_paged_cost[kWaves + 1]));
 
-  float* scratch = reinterpret_cast<float*>(A->scratch + A->task_scratch[ti]);
+  uint32_t* arrivals = reinterpret_cast<uint32_t*>(A->scratch + A->task_scratch[ti]);
+  float* scratch = reinterpret_cast<float*>(arrivals + kMaxLanes);
   const uint64_t slot_floats = paged_slot_floats(D);
-  uint32_t* arrivals = reinterpret_cast<uint32_t*>(scratch + 2 * uint64_t(W) * slot_floats);
 
   for (; s < D.B && base < c1; ++s) {
     PagedSeq q;

@@ -78,7 +78,8 @@ class PagedCache:
 class PagedBatch:
     """The rows of a step (``Graph.paged_batch``): sequence s's new tokens are rows
     cu[s] .. cu[s + 1] - 1, its length with them is lens[s], and position p of it
-    lies in page table[s, p // page]."""
+    lies in page table[s, p // page].  cu does not fall; a sequence that has rows
+    outside the step's is served as one whose length does not fit its rows."""
     cu: Tensor
     lens: Tensor
     table: Tensor
@@ -642,8 +643,8 @@ class Graph:
             raise GraphError(f"{what}: positions are i32 [{T}]")
         if weight is not None and (weight.shape != (hd,) or weight.dtype != V.DT_F32 or weight.view):
             raise GraphError(f"{what}: the norm's weight is f32 [{hd}]")
-        if not eps >= 0.0:
-            raise GraphError(f"{what}: eps is at least 0")
+        if not (eps >= 0.0 and math.isfinite(eps)):
+            raise GraphError(f"{what}: eps is finite and at least 0")
         return rot, self.const(turn_words(inv_freq), "u32")
 
     def rotary(self, x: Tensor, pos: Tensor, inv_freq, weight: Tensor | None = None, eps: float = 1e-6,

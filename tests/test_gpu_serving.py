@@ -201,6 +201,27 @@ def test_cache_append_special_rows():
         assert np.array_equal(np.isnan(got), np.isnan(w)) and np.array_equal(got[~np.isnan(w)], w[~np.isnan(w)])
 
 
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cache", ["f32", "f16", "bf16", "i8"])
+def test_cache_read_into_other_types(cache, out):
+    """Pages of every type read as every type, rounded once (f16's smallest steps are 2^-24;
+    an i8 value is a product rounded to f32 first)."""
+    dt = "bf16" if cache == "i8" else cache
+    c = SU.Case([(5, 30), (1, 9), (70, 100)], 3, 3, 40, 8, dt, cache, pad=1, seed=6)
+    g = G.Graph()
+    b, pc = c.declare(g)
+    g.output(*g.cache_read(pc, b, c.T, out))
+    kk, vv = compiled(g.build())(*c.batch(), *c.state())
+    for got, m in ((kk, 0), (vv, 1)):
+        ref = np.zeros(c.k.shape)
+        for i, (n, _) in enumerate(c.seqs):
+            ref[c.cu[i]:c.cu[i + 1]] = c.values(m, i)[0][-n:]
+        eps = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[out] + (2.0 ** -24 if cache == "i8" else 0.0)
+        if out == cache or out == "f32" and cache != "i8":
+            eps = 0.0
+        check(SU.to_f64(got, out), ref, eps * np.abs(ref) + (2.0 ** -25 if out == "f16" and eps else 0.0))
+
+
 def test_cache_append_from_views():
     """Keys and values inside the rows of a fused projection."""
     c = SU.Case([(19, 30), (4, 4)], 4, 2, 64, 16, "bf16")
@@ -310,6 +331,53 @@ def test_paged_attention_bad_batches(dt, cache, hd):
     check(SU.to_f64(got, dt), want, c.attention_tolerance(want, mag, top))
     out = SU.to_f64(got, dt)
     assert not out[0].any() and not out[c.cu[1]:c.cu[3]].any() and not out[c.cu[4]:].any()
+
+
+@pytest.mark.parametrize("cache", ["bf16", "i8"])
+def test_rows_outside_the_step(cache):
+    """A sequence whose rows reach past the step's, or lie before them, is not served: append
+    and read skip it, its rows' attention is 0."""
+    c = SU.Case([(4, 40), (6, 60), (5, 30)], 2, 2, 64, 16, "bf16", cache, seed=4)
+    state = c.state()
+    c.cu[0], c.cu[3] = -2, c.T + 3
+    g = G.Graph()
+    b, pc = c.declare(g)
+    g.cache_append(pc, b, g.input(c.k.shape, "bf16"), g.input(c.v.shape, "bf16"))
+    g.output(g.paged_attention(g.input(c.q.shape, "bf16"), pc, b, c.scale), *g.cache_read(pc, b, c.T, "f32"))
+    before = [x.copy() for x in state]
+    out, kk, vv = compiled(g.build())(*c.batch(), *state, c.k, c.v, c.q)
+    out, live = SU.to_f64(out, "bf16"), np.zeros(c.T, bool)
+    live[4:10] = True
+    for x in (out, kk, vv):
+        assert not x[~live].any() and x[live].any(axis=(1, 2)).all()
+    for i, n in ((0, range(36, 40)), (2, range(25, 30))):
+        for p in n:
+            pg, sl = slot_of(c, i, p)
+            for x, y in zip(state, before):
+                same(np.ascontiguousarray(x[pg, :, sl]), np.ascontiguousarray(y[pg, :, sl]))
+
+
+def test_attentions_of_other_shapes_share_scratch():
+    """Attention of several shapes in one program, each cut into pieces: their partials use the
+    same memory one after another, in every launch."""
+    cases = [SU.Case([(1, 40000)], 2, 1, 64, 64, "bf16", seed=1), SU.Case([(50, 9000), (1, 5000)], 8, 2, 128, 16, "bf16", seed=2),
+             SU.Case([(3, 7000)], 10, 5, 96, 16, "f32", seed=3)]
+    g = G.Graph()
+    ins, outs = [], []
+    for c in cases:
+        b, pc = c.declare(g)
+        q = g.input(c.q.shape, c.dt)
+        outs.append(g.paged_attention(q, pc, b, c.scale))
+        ins += [*c.batch(), *c.state(), c.q]
+    g.output(*outs)
+    lp = compiled(g.build())
+    first = lp(*ins)
+    for c, got in zip(cases, first):
+        want, mag, top = c.attention()
+        check(SU.to_f64(got, c.dt), want, c.attention_tolerance(want, mag, top))
+    for _ in range(3):
+        for got, was in zip(lp(*ins), first):
+            assert np.array_equal(got, was)
 
 
 @pytest.mark.parametrize("dt,cache,hd", [("bf16", "bf16", 128), ("f16", "f16", 64), ("f32", "f32", 64), ("bf16", "i8", 128),
