@@ -129,6 +129,13 @@ VM_DEV float head_sum(float x, uint32_t lph) {
   return x;
 }
 
+// 1 / sqrt(x), to an ulp; 0 and denormal x are scaled (the instruction takes them for 0).
+VM_DEV float inv_sqrt(float x) {
+  const bool small = x < 0x1p-120f;
+  const float r = __builtin_amdgcn_rsqf(small ? x * 0x1p+24f : x);
+  return small ? r * 0x1p+12f : r;
+}
+
 // The slots of a lane: NS at most (lane, lane + LPH, ...), their channels, weights and places
 // in the table of sines.
 template <int PW, int NS, bool INTER>
@@ -226,6 +233,30 @@ VM_DEV void rot_table(const RotDesc& D, float* tab, const VM_G int32_t* pos, con
 
 VM_DEV uint32_t pow2_at_least(uint32_t n) { return n <= 1 ? 1u : 1u << (32 - __builtin_clz(n - 1)); }
 
+// A lane's (row, head) pairs p0, p0 + by, ... of rows of `nh` heads, without a division each.
+// next(): row and head (past row nr - 1 of the last row), and whether it is within.
+struct RotPairs {
+  uint32_t r, h, dr, dh, nh;
+  VM_DEV RotPairs(uint32_t p0, uint32_t by, uint32_t heads) : nh(heads) {
+    r = p0 / nh;
+    h = p0 - r * nh;
+    dr = by / nh;
+    dh = by - dr * nh;
+  }
+  VM_DEV bool next(uint32_t nr, uint32_t* row, uint32_t* head) {
+    *row = min(r, nr - 1);
+    *head = h;
+    const bool in = r < nr;
+    h += dh;
+    r += dr;
+    if (h >= nh) {
+      h -= nh;
+      ++r;
+    }
+    return in;
+  }
+};
+
 // A lane's raw runs of N steps: x, or dy and then x.
 template <uint32_t DT, int PW, int NS, bool GRAD = false>
 struct RotBatch {
@@ -244,27 +275,24 @@ struct RotBatch {
 template <template <int> class Batch, int KB, class Load, class Compute, class Before>
 VM_DEV void rot_steps(uint32_t n, uint32_t hpw, Load load, Compute compute, Before before) {
   const uint32_t steps = (n + hpw - 1) / hpw, full = n / hpw / KB;
-  if (full) {
-    Batch<KB> b0, b1;
-    load(0, b0);
-    before();
-    for (uint32_t b = 0; b < full; b += 2) {
-      if (b + 1 < full) load((b + 1) * KB, b1);
-      compute(b * KB, b0);
-      if (b + 1 >= full) break;
-      if (b + 2 < full) load((b + 2) * KB, b0);
-      compute((b + 1) * KB, b1);
-    }
-  }
-  uint32_t s = full * KB;
-  if (s >= steps) return;
+  Batch<KB> b0, b1;
   Batch<1> b;
-  load(s, b);
-  if (!full) before();
-  for (;;) {
+  if (full) load(0, b0);
+  else load(0, b);
+  before();
+  if (full) {
+    for (uint32_t i = 0; i < full; i += 2) {
+      if (i + 1 < full) load((i + 1) * KB, b1);
+      compute(i * KB, b0);
+      if (i + 1 >= full) break;
+      if (i + 2 < full) load((i + 2) * KB, b0);
+      compute((i + 1) * KB, b1);
+    }
+    if (full * KB < steps) load(full * KB, b);
+  }
+  for (uint32_t s = full * KB; s < steps; ++s) {
     compute(s, b);
-    if (++s >= steps) break;
-    load(s, b);
+    if (s + 1 < steps) load(s + 1, b);
   }
 }
 
@@ -292,17 +320,13 @@ VM_DEV void rotary_units(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
   // rows [row, row + nr), heads [h0, h1)
   auto unit = [&](uint32_t row, uint32_t nr, uint32_t h0, uint32_t h1) {
     const uint32_t nh = h1 - h0, n = nr * nh;
-    // pair `s hpw + hg`: the lane's row (of the unit) and head; past the last it is the last
-    auto which = [&](uint32_t s, uint32_t* r, uint32_t* h) {
-      const uint32_t p = min(s * hpw + hg, n - 1);
-      *r = p / nh;
-      *h = h0 + p - *r * nh;
-    };
+    RotPairs pl(hg, hpw, nh), ps = pl;
     auto load = [&](uint32_t s0, auto& B) {
 #pragma unroll
       for (int k = 0; k < B.kN; ++k) {
         uint32_t r, h;
-        which(s0 + k, &r, &h);
+        pl.next(nr, &r, &h);
+        h += h0;
         const uint64_t e = uint64_t(row + r) * D.ars + uint64_t(h) * D.ahs + D.aoff;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -315,8 +339,8 @@ VM_DEV void rotary_units(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
 #pragma unroll
       for (int k = 0; k < B.kN; ++k) {
         uint32_t r, h;
-        which(s0 + k, &r, &h);
-        const bool in = (s0 + k) * hpw + hg < n;
+        const bool in = ps.next(nr, &r, &h);
+        h += h0;
         float z = 1.0f;
         if (norm) {
           float ss = 0.0f;
@@ -327,7 +351,7 @@ VM_DEV void rotary_units(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
               const float a = S.on[s] ? B.r0[k][s].get(i) : 0.0f, c = S.on[s] ? B.r1[k][s].get(i) : 0.0f;
               ss = fmaf(a, a, fmaf(c, c, ss));
             }
-          z = 1.0f / sqrtf(fmaf(head_sum(ss, lph), inv_hd, D.eps));
+          z = inv_sqrt(fmaf(head_sum(ss, lph), inv_hd, D.eps));
         }
         const uint64_t e = (uint64_t(row + r) * D.H + h) * D.hd;
 #pragma unroll
@@ -359,17 +383,16 @@ VM_DEV void rotary_units(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
     rot_steps<RotBatch<DT, PW, NS>::template X, KB>(n, hpw, load, compute,
                                                     [&] { rot_table(D, tab, pos, freq, row, nr, PW, sign); });
   };
-  if (Z == 1) {
-    // tile: four rows; a wave's quarter of the entry's rows, kRotRows at a time
-    const uint32_t r0 = 4 * lo, rows = min(D.T, 4 * hi) - r0;
-    uint32_t r = r0 + rows * wave / 4;
-    const uint32_t end = r0 + rows * (wave + 1) / 4;
-    for (; r < end; r += kRotRows) unit(r, min(kRotRows, end - r), 0, D.H);
-    return;
+  // Z = 1: a tile is four rows, a wave takes its quarter of the entry's rows, kRotRows at a
+  // time; else four (row, split) pairs, a wave every fourth
+  const uint32_t n0 = 4 * lo, rows = min(D.T * Z, 4 * hi) - n0, hz = (D.H + Z - 1) / Z;   // heads of a split
+  uint32_t u = n0 + (Z == 1 ? rows * wave / 4 : wave);
+  const uint32_t end = Z == 1 ? n0 + rows * (wave + 1) / 4 : n0 + rows;
+  while (u < end) {
+    const uint32_t nr = Z == 1 ? min(kRotRows, end - u) : 1, h0 = Z == 1 ? 0 : u % Z * hz;
+    if (h0 < D.H) unit(Z == 1 ? u : u / Z, nr, h0, min(D.H, h0 + hz));
+    u += Z == 1 ? nr : 4;
   }
-  const uint32_t hz = (D.H + Z - 1) / Z;                        // heads of a split
-  for (uint32_t u = 4 * lo + wave; u < min(4 * hi, D.T * Z); u += 4)
-    if (u % Z * hz < D.H) unit(u / Z, 1, u % Z * hz, min(D.H, u % Z * hz + hz));
 }
 
 // Worker `tile` of p3: a contiguous share of the (row, head) pairs, a quarter of it a wave,
@@ -409,16 +432,14 @@ VM_DEV void rotary_grad_worker(Args A, uint32_t ti, uint32_t tile) {
     const uint32_t row = at / H, last = uint32_t(min(uint64_t(end), uint64_t(row + kRotRows) * H));
     const uint32_t first = at - row * H, n = last - at;         // pairs `first` .. of the rows from `row`
     at = last;
-    auto which = [&](uint32_t s, uint32_t* r, uint32_t* h) {
-      const uint32_t p = first + min(s * hpw + hg, n - 1);
-      *r = p / H;
-      *h = p - *r * H;
-    };
+    // (rows past the last pair's are the next wave's, or not there: `in` counts pairs)
+    RotPairs pl(first + hg, hpw, H), ps = pl;
+    const uint32_t nr = (first + n - 1) / H + 1;
     auto load = [&](uint32_t s0, auto& B) {
 #pragma unroll
       for (int k = 0; k < B.kN; ++k) {
         uint32_t r, h;
-        which(s0 + k, &r, &h);
+        pl.next(nr, &r, &h);
         const uint64_t ye = uint64_t(row + r) * D.ars + uint64_t(h) * D.ahs + D.aoff;
         const uint64_t xe = uint64_t(row + r) * D.brs + uint64_t(h) * D.bhs + D.boff;
 #pragma unroll
@@ -434,7 +455,7 @@ VM_DEV void rotary_grad_worker(Args A, uint32_t ti, uint32_t tile) {
 #pragma unroll
       for (int k = 0; k < B.kN; ++k) {
         uint32_t r, h;
-        which(s0 + k, &r, &h);
+        ps.next(nr, &r, &h);
         const bool in = (s0 + k) * hpw + hg < n;
         float ss = 0.0f, dot = 0.0f;
         float za[NS][PW], zb[NS][PW], xa[NS][PW], xb[NS][PW];
@@ -456,7 +477,7 @@ VM_DEV void rotary_grad_worker(Args A, uint32_t ti, uint32_t tile) {
             dot = fmaf(za[s][i] * wa, xa[s][i], fmaf(zb[s][i] * wb, xb[s][i], dot));
           }
         }
-        const float z = 1.0f / sqrtf(fmaf(head_sum(ss, lph), inv_hd, D.eps));
+        const float z = inv_sqrt(fmaf(head_sum(ss, lph), inv_hd, D.eps));
         const float c = z * z * z * (head_sum(dot, lph) * inv_hd);
         const uint64_t e = (uint64_t(row + r) * H + h) * D.hd;
 #pragma unroll
@@ -556,7 +577,7 @@ VM_DEV void rotary_grad_worker(Args A, uint32_t ti, uint32_t tile) {
 }
 
 template <uint32_t DT, int PW, int NS, bool INTER>
-VM_TILE void rotary_run(Args A, uint32_t ti, uint32_t lo, uint32_t hi, bool grad) {
+VM_LEAF void rotary_run(Args A, uint32_t ti, uint32_t lo, uint32_t hi, bool grad) {
   A = uargs(A);
   lo = uni(lo);
   hi = uni(hi);
