@@ -104,7 +104,9 @@ int vmrt_program_io(vmrt_program* prog, int is_output, uint32_t index, uint32_t*
 /* Run the program on device buffers: inputs are read in place and outputs
  * written in place (zero-copy ports), then wait for completion and check the VM
  * status word.  Replaces LoadedProgram::ExecuteDevice (runtime.h:340-346;
- * runtime.cc:2107-2242). */
+ * runtime.cc:2107-2242).  A state input (a paged cache; no counterpart in the
+ * reference) is written in place: every launch refuses one that is not 16-byte
+ * aligned or shares memory with another input or output. */
 int vmrt_execute(vmrt_program* prog, const void* const* inputs, size_t n_inputs, void* const* outputs,
                  size_t n_outputs, char* err, size_t errlen);
 
