@@ -25,7 +25,11 @@
 // not hold the scales' range).
 //
 // P is rounded to the type of the second product (bf16 / f16: half a step, 2^-8 / 2^-11
-// of each weight, the row sum taken over the rounded weights); everything else is f32.
+// of each weight, the row sum taken over the rounded weights); everything else is f32.  With
+// f16 queries over i8 pages P is the sum of two bf16 numbers (2^-16) and the second product
+// is done twice, since one bf16 would cost the output eight times its own rounding (a chunk of
+// 2048 rows over 8192 keys 546 us, with bf16 queries and one product 447; 256-row blocks spill
+// a little there, 276 B a lane, and 128-row ones take 659).
 //
 // Positions that a row does not see weigh 0, and those outside the piece or without a page
 // are zeros in LDS.  A position that one row of the block sees and another does not may
@@ -119,6 +123,32 @@ VM_DEV float frag_sum(const u16x8& f) {
   return dot2_ones<BF16>(w.w, dot2_ones<BF16>(w.z, dot2_ones<BF16>(w.y, dot2_ones<BF16>(w.x, 0.0f))));
 }
 
+// A fragment of P, in two parts where one bf16 is not enough.
+template <bool TWO>
+struct PFrag {
+  u16x8 hi;
+};
+template <>
+struct PFrag<true> {
+  u16x8 hi, lo;
+};
+// Eight weights as a fragment; returns the sum of what it holds.
+template <bool PBF, bool TWO>
+VM_DEV float pack_p(const float (&e)[8], PFrag<TWO>& f) {
+  const v4u w = v4u_make(pack_h2<PBF>(e[0], e[1]), pack_h2<PBF>(e[2], e[3]), pack_h2<PBF>(e[4], e[5]), pack_h2<PBF>(e[6], e[7]));
+  f.hi = __builtin_bit_cast(u16x8, w);
+  float sum = frag_sum<PBF>(f.hi);
+  if constexpr (TWO) {
+    float d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = e[i] - __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    PFrag<false> lo;
+    sum += pack_p<PBF>(d, lo);
+    f.lo = lo.hi;
+  }
+  return sum;
+}
+
 // What both forms share: a block's rows, its keys' rows in the pages, and the products of
 // one 32-key half.
 template <int HD, bool BF16, bool Q8, int U>
@@ -127,6 +157,13 @@ struct PagedMma {
   static constexpr uint32_t kES = Q8 ? 1 : 2;
   static constexpr uint32_t kRow = HD * kES;                   // LDS bytes of a key row
   static constexpr bool PBF = BF16 || Q8;                      // type of the second product
+  static constexpr bool P2 = !BF16 && Q8;
+  typedef PFrag<P2> Pf;
+  VM_DEV static f32x16 pv_mma(const u16x8& v, const Pf& p, f32x16 o) {
+    o = mfma16<PBF>(v, p.hi, o);
+    if constexpr (P2) o = mfma16<PBF>(v, p.lo, o);
+    return o;
+  }
 
   const PagedDesc& D;
   const PagedJob& J;
@@ -268,7 +305,7 @@ struct PagedMma {
   }
   // P of a half against the reference mu: two fragments, the row sums and (i8) the sums of
   // the rounded P vs
-  VM_DEV void probs(const f32x16& s, float mu, const lds_u8* vs, u16x8& pf0, u16x8& pf1, float& rs, float& ps) {
+  VM_DEV void probs(const f32x16& s, float mu, const lds_u8* vs, Pf& pf0, Pf& pf1, float& rs, float& ps) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       float e[8];
@@ -282,10 +319,7 @@ struct PagedMma {
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = e[i] == 0.0f ? 0.0f : e[i] * (i < 4 ? x0[i & 3] : x1[i & 3]);
       }
-      const v4u w = v4u_make(pack_h2<PBF>(e[0], e[1]), pack_h2<PBF>(e[2], e[3]), pack_h2<PBF>(e[4], e[5]),
-                             pack_h2<PBF>(e[6], e[7]));
-      (ks ? pf1 : pf0) = __builtin_bit_cast(u16x8, w);
-      const float sum = dot2_ones<PBF>(w.w, dot2_ones<PBF>(w.z, dot2_ones<PBF>(w.y, dot2_ones<PBF>(w.x, 0.0f))));
+      const float sum = pack_p<PBF>(e, ks ? pf1 : pf0);
       if constexpr (Q8) ps += sum;
       else rs += sum;
     }
@@ -416,7 +450,7 @@ VM_LEAF bool paged_block_wave(Args A, uint32_t ti, PagedJob J) {
     }
     u16x8 kf[M::KS];
     f32x16 sv[U];
-    u16x8 pf[U][2];
+    typename M::Pf pf[U][2];
     B.k_frags(K, kf);
 #pragma unroll
     for (int u = 0; u < U; ++u) B.scores(K, u, sv[u], kf);
@@ -438,7 +472,7 @@ VM_LEAF bool paged_block_wave(Args A, uint32_t ti, PagedJob J) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int db = 0; db < M::DB; ++db) B.o[u][db] = mfma16<M::PBF>(vf[db], pf[u][ks], B.o[u][db]);
+        for (int db = 0; db < M::DB; ++db) B.o[u][db] = M::pv_mma(vf[db], pf[u][ks], B.o[u][db]);
     }
    }
    if (j < nb) {
@@ -684,9 +718,8 @@ VM_LEAF bool paged_block_few(Args A, uint32_t ti, PagedJob J) {
 #pragma unroll
           for (int x = 0; x < 8; ++x) e[x] = (there >> (8 * q + x)) & 1 ? e[x] : 0.0f;
       }
-      const v4u w = v4u_make(pack_h2<PBF>(e[0], e[1]), pack_h2<PBF>(e[2], e[3]), pack_h2<PBF>(e[4], e[5]), pack_h2<PBF>(e[6], e[7]));
-      const u16x8 pf = __builtin_bit_cast(u16x8, w);
-      const float ps = frag_sum<PBF>(pf);
+      PFrag<!BF16 && Q8> pf;
+      const float ps = pack_p<PBF>(e, pf);
       if constexpr (Q8) pv += ps;
       else l += ps;
 #pragma unroll
@@ -703,7 +736,8 @@ VM_LEAF bool paged_block_few(Args A, uint32_t ti, PagedJob J) {
           const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * W::kRow));
           vf = __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
-        o[x] = mfma16x16<PBF>(vf, pf, o[x]);
+        o[x] = mfma16x16<PBF>(vf, pf.hi, o[x]);
+        if constexpr (!BF16 && Q8) o[x] = mfma16x16<PBF>(vf, pf.lo, o[x]);
       }
     }
     if (j < nb) {
@@ -828,7 +862,7 @@ VM_LEAF bool paged_block_rows(Args A, uint32_t ti, PagedJob J) {
         *(lds_v4u_t*)(uintptr_t)(lds0 + (kb & 1) * W::kStage + W::kOp + 4096 * j + in) = v4u_make(0, 0, 0, 0);
   };
   // A masked block (and every one of a careful sweep): the online update.
-  auto online = [&](int u, f32x16 (&s)[2], uint32_t ka, uint64_t there, const lds_u8* sc, u16x8 (&pf)[4]) {
+  auto online = [&](int u, f32x16 (&s)[2], uint32_t ka, uint64_t there, const lds_u8* sc, typename M::Pf (&pf)[4]) {
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
       B.key_scales(s[kh], u, sc + 128 * kh);
@@ -847,7 +881,7 @@ VM_LEAF bool paged_block_rows(Args A, uint32_t ti, PagedJob J) {
   // swept again, carefully.
   const float bound = M::PBF ? 16777216.0f : 16384.0f;
   bool again = false;
-  auto fixed = [&](int u, f32x16 (&s)[2], const lds_u8* sc, u16x8 (&pf)[4]) {
+  auto fixed = [&](int u, f32x16 (&s)[2], const lds_u8* sc, typename M::Pf (&pf)[4]) {
     float rs = 0.0f;
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
@@ -878,7 +912,7 @@ VM_LEAF bool paged_block_rows(Args A, uint32_t ti, PagedJob J) {
           for (int kh = 0; kh < 2; ++kh) s1[kh] = mfma16<BF16>(kf[kh][st], B.qf[1][st], s1[kh]);
       }
     }
-    u16x8 p0[4], p1[4];
+    typename M::Pf p0[4], p1[4];
     if constexpr (decltype(maskedc)::value) online(0, s0, ka, there, sc, p0);
     else fixed(0, s0, sc, p0);
     u16x8 vf[4][M::DB];
@@ -887,14 +921,14 @@ VM_LEAF bool paged_block_rows(Args A, uint32_t ti, PagedJob J) {
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-      for (int db = 0; db < M::DB; ++db) B.o[0][db] = mfma16<M::PBF>(vf[ks][db], p0[ks], B.o[0][db]);
+      for (int db = 0; db < M::DB; ++db) B.o[0][db] = M::pv_mma(vf[ks][db], p0[ks], B.o[0][db]);
     if constexpr (U == 2) {
       if constexpr (decltype(maskedc)::value) online(1, s1, ka, there, sc, p1);
       else fixed(1, s1, sc, p1);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-        for (int db = 0; db < M::DB; ++db) B.o[1][db] = mfma16<M::PBF>(vf[ks][db], p1[ks], B.o[1][db]);
+        for (int db = 0; db < M::DB; ++db) B.o[1][db] = M::pv_mma(vf[ks][db], p1[ks], B.o[1][db]);
     }
   };
   // blocks [f0, f1) that every row of the wave sees whole

@@ -123,12 +123,13 @@ class Case:
         """Per element: rounding P, the output's rounding, and f32 sums.  P is rounded to the
         queries' type, w (1 + d) with |d| <= half a step, and divided by the sum of the
         rounded ones: 2 half steps of sum w |v|.  Over i8 pages P times the value's scale is
-        rounded to bf16 (f16 has no room for the scales' range) and divided by the sum of
-        the unrounded P: sum w (1 + d) v with |d| <= 2^-8 is off by at most 2^-8 sum w |v|.
+        rounded to bf16 (f16 has no room for the scales' range; with f16 queries to the sum
+        of two bf16 numbers, so |d| <= 2^-8 2^-8) and divided by the sum of the unrounded P:
+        sum w (1 + d) v with |d| <= 2^-8 is off by at most 2^-8 sum w |v|.
         The sums: a score is off by at most (hd + 4) 2^-24 of sum |q k| scale, taken as 4
         times the largest score, which moves every weight by that factor; exp2, the
         sums and the division add at most 64 2^-24."""
-        p = 0.0 if self.dt == "f32" else U["bf16"] if self.cache == "i8" else U[self.dt]
+        p = 0.0 if self.dt == "f32" else (U["bf16"] if self.dt == "bf16" else U["bf16"] ** 2) if self.cache == "i8" else U[self.dt]
         f32 = ((self.hd + 4) * 4 * top + 64 + 2 * top) * 2.0 ** -24
         return (2 * p + 2 * f32) * mag + U[self.dt] * np.abs(out) + 1e-30
 
