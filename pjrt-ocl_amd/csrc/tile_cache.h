@@ -19,6 +19,9 @@
 // the tile's (row, k or v, head) rows: 16 loads in flight a lane (of f32 eight), kept in LDS while
 // the next are on their way and a short loop stores them (one that is unrolled over as many
 // rows took as long: every lane runs it once, as fast as its instructions come from memory).
+// 4096 rows of 8 heads of 128 from bf16: into bf16 pages 5.8 us a lane (33.5 MB: HBM), into i8
+// pages 11 (the conversion's instructions), out of those into f32 13 (42 MB, and 3.5 us until
+// the first loads have their rows' places).
 #pragma once
 #include "tile_rotary.h"
 #include "vm_divu32.h"

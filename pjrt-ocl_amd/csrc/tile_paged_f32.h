@@ -9,7 +9,8 @@
 //   O^T (16 channels x 16 rows) += V^T P^T: step i takes key 4 q + i, the key that the
 //   lane's accumulator i of S^T holds, so P^T is those registers.
 // A block of 64 rows does 16 flops a byte of LDS and is bound by the matrix cores (f32: a
-// sixteenth of bf16's rate); a few rows by HBM.
+// sixteenth of bf16's rate); a few rows by HBM.  Five sequences of 7 rows and 350 to 1050 keys,
+// 8 / 4 heads of 96: 38 us (176 with a wave a row), most of it one item's latency.
 #pragma once
 #include "tile_paged_mma.h"
 

@@ -20,8 +20,11 @@
 // kRotRows rows at a time: their sines go into LDS once (a pair a lane, 35 instructions each; each
 // lane working its own eight pairs out for every row took 48 of 99 us for 8192 rows of 40
 // heads), then the (row, head) pairs pass in batches, the next batch's loads in flight
-// while one is computed (there is one wave per SIMD to hide them).  Both operators are bound
-// by HBM: x is read and y written once.
+// while one is computed (there is one wave per SIMD to hide them).  x is read and y written
+// once: 8192 rows of 40 heads of 128, bf16 with the norm, 168 MB in 45 us (3.75 TB/s), the
+// gradient of 4096 rows of 32 heads, 101 MB in 36.  What is left beside HBM is instruction
+// issue, some 150 instructions for a lane's 16 channels: larger batches change nothing, and
+// a division less for each pair and the hardware's 1 / sqrt took 4 %.
 #pragma once
 #include "vm_device.h"
 

@@ -1215,7 +1215,7 @@ class _Scheduler:
             if t.tile_op == V.TOP_ROTARY:
                 # queries and keys of the same rows: each lane takes its share of both, so
                 # that they end together (8192 rows of 32 and 8 heads: 75 us in chunks of
-                # their own, with 2 of 256 tiles on a third of the lanes)
+                # their own, with 2 of 256 tiles on a third of the lanes, 56 so)
                 tiles, cost = n_tiles(t, self.cfg), task_cost(t, self.cfg, self.prog)
                 if tiles in rotary:
                     u = rotary[tiles]
