@@ -175,7 +175,7 @@ VM_DEV void i8_rows(const Run<DT, 8> (&x)[V], uint32_t lph, float (&scale)[V], v
 
 // DT: the rows' element type; Q8: pages of i8 (else of DT).  READ: out of the pages.
 template <uint32_t DT, bool Q8, bool READ>
-VM_LEAF void cache_move(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
+VM_TILE void cache_move(Args A, uint32_t ti, uint32_t lo, uint32_t hi) {
   A = uargs(A);
   lo = uni(lo);
   hi = uni(hi);

@@ -21,10 +21,11 @@
 // lane working its own eight pairs out for every row took 48 of 99 us for 8192 rows of 40
 // heads), then the (row, head) pairs pass in batches, the next batch's loads in flight
 // while one is computed (there is one wave per SIMD to hide them).  x is read and y written
-// once: 8192 rows of 40 heads of 128, bf16 with the norm, 168 MB in 45 us (3.75 TB/s), the
-// gradient of 4096 rows of 32 heads, 101 MB in 36.  What is left beside HBM is instruction
+// once: 8192 rows of 40 heads of 128, bf16 with the norm, 168 MB in 48 us (3.5 TB/s), the
+// gradient of 4096 rows of 32 heads, 101 MB in 39.  What is left beside HBM is instruction
 // issue, some 150 instructions for a lane's 16 channels: larger batches change nothing, and
-// a division less for each pair and the hardware's 1 / sqrt took 4 %.
+// a division less for each pair and the hardware's 1 / sqrt took 4 %.  As leaves they take 2 to
+// 4 us less, but then the kernel saves more around every call: a decoder's steps took 3 % longer.
 #pragma once
 #include "vm_device.h"
 
@@ -580,7 +581,7 @@ VM_DEV void rotary_grad_worker(Args A, uint32_t ti, uint32_t tile) {
 }
 
 template <uint32_t DT, int PW, int NS, bool INTER>
-VM_LEAF void rotary_run(Args A, uint32_t ti, uint32_t lo, uint32_t hi, bool grad) {
+VM_TILE void rotary_run(Args A, uint32_t ti, uint32_t lo, uint32_t hi, bool grad) {
   A = uargs(A);
   lo = uni(lo);
   hi = uni(hi);
